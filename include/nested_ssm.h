@@ -62,7 +62,7 @@
 extern "C" {
 #endif
 
-#define NSSM_ABI_VERSION 3
+#define NSSM_ABI_VERSION 4
 
 #if defined(__GNUC__)
 #define NSSM_API __attribute__((visibility("default")))
@@ -382,6 +382,163 @@ NSSM_API int nssm_verify_step(const nssm_pool* pool, const nssm_step_args* args,
  * nssm_spec_workspace_bytes() bytes is always needed. */
 NSSM_API int nssm_commit_step(const nssm_pool* pool, const nssm_step_args* args, const nssm_token_args* tok,
                               void* stream);
+
+/* ---- gated delta rule ---------------------------------------------------------------------
+ * The recurrent state rule of gated delta layers on states of the same layout as the untiered
+ * state update, per value head h with key group j = h / (nheads / ngroups):
+ *   S <- exp(g) S;  u = beta (v - S k);  S <- S + u k^T;  y = scale S q
+ * S [headdim][dstate] fp32, q and k [dstate], v and y [headdim].  Beside nssm_fresh_step (decode)
+ * and nssm_chunk_scan (prefill); no counterpart in the reference, whose models have no such
+ * layers.  Compiled for dstate 64 and 128, headdim a multiple of 16 up to 256. */
+
+/* Device status bit 3, of the calls below: a slot named twice, a sequence whose bounds are not
+ * ascending inside the tokens, or a slot move that would read a slot another move writes. */
+#define NSSM_STATUS_CONFLICT 8
+
+typedef struct {
+  int32_t batch, num_slots, nheads, ngroups, headdim, dstate;
+  int32_t io_dtype;       /* dtype of q, k, v (F32 or BF16)                          */
+  int32_t g_dtype;        /* F32 or BF16                                             */
+  int32_t beta_dtype;     /* F32 or BF16                                             */
+  int32_t out_dtype;      /* F32 or BF16                                             */
+  int32_t pad_slot_id;    /* rows with this slot are skipped                         */
+  float scale;
+  float* state;           /* [num_slots][nheads][headdim][dstate], updated in place  */
+  int64_t state_stride_s; /* a multiple of 4                                         */
+  const void* q;          /* [batch][ngroups][dstate], any alignment                 */
+  int64_t q_stride_b, q_stride_h;
+  const void* k;
+  int64_t k_stride_b, k_stride_h;
+  const void* v;          /* [batch][nheads][headdim]                                */
+  int64_t v_stride_b, v_stride_h;
+  const void* g;          /* [batch][nheads]: log of the decay                       */
+  int64_t g_stride_b, g_stride_h;
+  const void* beta;       /* [batch][nheads]                                         */
+  int64_t beta_stride_b, beta_stride_h;
+  const int32_t* state_batch_indices; /* [batch] slot of each row; NULL = row        */
+  void* out;              /* [batch][nheads][headdim]                                */
+  int64_t out_stride_b, out_stride_h;
+  int32_t* status;        /* optional device word: bit 0 slot out of range, bit 3 a slot named
+                             by an earlier row of the batch (the later row is skipped)  */
+} nssm_delta_step_args;
+
+/* One decode token per row. */
+NSSM_API int nssm_delta_step(const nssm_delta_step_args* args, void* stream);
+NSSM_API size_t nssm_sizeof_delta_step_args(void);
+
+/* Prompts: y of every token and the state after the last one.  With cu_seqlens the batch is
+ * packed: sequence s has the tokens cu_seqlens[s] .. cu_seqlens[s+1] of one row of `seqlen`
+ * tokens (the _b strides of the inputs are not used); tokens outside every sequence are not
+ * read, and their y is not written.  q, k, v, y bf16; token strides multiples of 8 elements,
+ * bases 16-byte aligned; (group, dstate) and (head, headdim) packed; heads of g and beta packed. */
+typedef struct {
+  int32_t batch;          /* sequences                                               */
+  int32_t seqlen;         /* tokens of each, or of all when cu_seqlens is given      */
+  int32_t nheads, ngroups, headdim, dstate;
+  int32_t g_dtype, beta_dtype;
+  float scale;
+  int32_t _pad0;
+  const void* q;          /* [batch][seqlen][ngroups][dstate] bf16                   */
+  int64_t q_stride_b, q_stride_t;
+  const void* k;
+  int64_t k_stride_b, k_stride_t;
+  const void* v;          /* [batch][seqlen][nheads][headdim] bf16                   */
+  int64_t v_stride_b, v_stride_t;
+  const void* g;          /* [batch][seqlen][nheads]                                 */
+  int64_t g_stride_b, g_stride_t;
+  const void* beta;
+  int64_t beta_stride_b, beta_stride_t;
+  const int32_t* cu_seqlens; /* [batch + 1] or NULL                                  */
+  const float* initial_states; /* [batch][nheads][headdim][dstate] or NULL (zeros)   */
+  int64_t init_stride_b;
+  void* y;                /* [batch][seqlen][nheads][headdim] bf16                   */
+  int64_t y_stride_b, y_stride_t;
+  float* final_states;    /* [batch][nheads][headdim][dstate] or NULL; may be initial_states */
+  int64_t final_stride_b;
+  void* workspace;        /* nssm_delta_scan_workspace_bytes()                       */
+  size_t workspace_bytes;
+  int32_t* status;        /* optional device word, bit 3 = bad cu_seqlens (that sequence is skipped) */
+} nssm_delta_scan_args;
+
+NSSM_API size_t nssm_delta_scan_workspace_bytes(int32_t batch, int32_t seqlen, int32_t nheads, int32_t headdim,
+                                                int32_t dstate, int32_t packed);
+NSSM_API int nssm_delta_scan(const nssm_delta_scan_args* args, void* stream);
+NSSM_API size_t nssm_sizeof_delta_scan_args(void);
+
+/* ---- moves of slots -----------------------------------------------------------------------
+ * A slot's state may lie in several buffers (the buffers of a pool, conv states, every layer of
+ * each); a move takes them all.  The list of moves is checked on the device before anything is
+ * written: a slot out of range (bit 0 of *status), a destination named twice or a destination
+ * that another move reads (bit 3) drops those moves and no others, so the result does not depend
+ * on the order of execution.  A move of a slot onto itself does nothing. */
+typedef struct {
+  void* base;             /* element (o, s, 0) at base + o*outer_stride + s*slot_stride, bytes */
+  int64_t outer_stride;
+  int64_t slot_stride;
+  int64_t row_bytes;      /* contiguous bytes of one slot                            */
+  int32_t outer;          /* layers                                                  */
+  int32_t _pad0;
+} nssm_slot_buffer;
+
+#define NSSM_MAX_SLOT_BUFFERS 24
+#define NSSM_MAX_SLOT_ROWS 4096     /* rows of one call                               */
+#define NSSM_MAX_MOVE_SLOTS 131072  /* slots of a buffer                              */
+
+NSSM_API size_t nssm_sizeof_slot_buffer(void);
+NSSM_API size_t nssm_slot_workspace_bytes(int32_t rows);
+
+/* dst[i] <- src[i] in every buffer (the same src may be named many times: a fork); entries whose
+ * src or dst is pad_slot_id are skipped.  src NULL: dst[i] <- zero bytes (a freed slot).
+ * `bufs` is a host array. */
+NSSM_API int nssm_slot_copy(const nssm_slot_buffer* bufs, int32_t nbuf, int32_t num_slots, const int32_t* src,
+                            const int32_t* dst, int32_t rows, int32_t pad_slot_id, void* workspace,
+                            size_t workspace_bytes, int32_t* status, void* stream);
+
+/* Row r continues row parents[r] (within its group of `group` rows; group == rows for indices over
+ * the whole batch).  The first child of a parent keeps the parent's slot, every other child takes
+ * the slot of a row without children, in row order, and the parent's state is copied there: the
+ * fewest copies.  new_slots [rows].  A row whose parent is padded becomes padded. */
+NSSM_API int nssm_slot_reorder(const nssm_slot_buffer* bufs, int32_t nbuf, int32_t num_slots, const int32_t* slots,
+                               const int32_t* parents, int32_t rows, int32_t group, int32_t pad_slot_id,
+                               int32_t* new_slots, void* workspace, size_t workspace_bytes, int32_t* status,
+                               void* stream);
+
+/* The m live slots move into slots 0 .. m-1: those below m stay, the others take the free ones
+ * below m in row order.  new_slots [rows]. */
+NSSM_API int nssm_slot_compact(const nssm_slot_buffer* bufs, int32_t nbuf, int32_t num_slots, const int32_t* slots,
+                               int32_t rows, int32_t pad_slot_id, int32_t* new_slots, void* workspace,
+                               size_t workspace_bytes, int32_t* status, void* stream);
+
+/* ---- beam search ----------------------------------------------------------------------------
+ * The nout best continuations of each prompt's beams: total = scores[b][j] + x - log sum exp(x)
+ * over a beam's logits x.  Candidates of one beam rank by logit, then by the lower token; those
+ * of different beams by total (64-bit), then by the lower beam.  A logit that is not finite
+ * counts as masked: it adds nothing to the sum and its total is -inf; a total that is not a number
+ * is -inf.  A finished beam has one continuation, eos_token at its own score.  Beside the state
+ * moves above, which then give each continuation its state. */
+typedef struct {
+  int32_t batch, beams, vocab, nout;
+  int32_t logits_dtype;   /* F32 or BF16                                             */
+  int32_t eos_token;      /* < 0: none                                               */
+  const void* logits;     /* [batch][beams][vocab], any alignment                    */
+  int64_t logits_stride_b, logits_stride_k;
+  const float* scores;    /* [batch][beams]                                          */
+  const uint8_t* finished; /* [batch][beams] or NULL                                 */
+  float* out_scores;      /* [batch][nout], descending                               */
+  int32_t* out_parents;   /* [batch][nout] beam that is continued                    */
+  int32_t* out_tokens;    /* [batch][nout]                                           */
+  uint8_t* out_finished;  /* [batch][nout] or NULL                                   */
+  void* workspace;
+  size_t workspace_bytes;
+} nssm_beam_args;
+
+#define NSSM_MAX_BEAMS 64
+#define NSSM_MAX_BEAM_OUT 128
+
+NSSM_API size_t nssm_beam_workspace_bytes(int32_t batch, int32_t beams, int32_t vocab, int32_t nout,
+                                          int32_t logits_dtype);
+NSSM_API int nssm_beam_select(const nssm_beam_args* args, void* stream);
+NSSM_API size_t nssm_sizeof_beam_args(void);
 
 /* sizeof of the argument structs, for binding checks. */
 NSSM_API size_t nssm_sizeof_pool(void);

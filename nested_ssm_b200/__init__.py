@@ -22,6 +22,9 @@ from .ops import (  # noqa: F401
     tiered_state_update,
     verify_state_update,
 )
+from .beam import beam_select  # noqa: F401
+from .delta import gated_delta_chunk_scan, gated_delta_state_update  # noqa: F401
 from .pool import TieredSlotPool  # noqa: F401
+from .slots import StateBuffers, clear_slots, compact_slots, copy_slots, reorder_slots  # noqa: F401
 
 __version__ = "0.1.0"

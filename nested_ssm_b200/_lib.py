@@ -15,7 +15,8 @@ from . import build as _build
 NSSM_OK, NSSM_ERR_INVALID, NSSM_ERR_UNSUPPORTED, NSSM_ERR_CUDA = 0, 1, 2, 3
 NSSM_F32, NSSM_BF16, NSSM_F8E4M3 = 0, 1, 2
 NSSM_MODE_STALE, NSSM_MODE_CORR, NSSM_MODE_COLDOFF = 0, 1, 2
-ABI_VERSION = 3
+NSSM_STATUS_CONFLICT = 8
+ABI_VERSION = 4
 
 EXPORTED = (
     "nssm_step_workspace_bytes", "nssm_tiered_step", "nssm_fresh_step", "nssm_prefill_split",
@@ -24,7 +25,10 @@ EXPORTED = (
     "nssm_conv_step", "nssm_sizeof_conv_args", "nssm_gated_rmsnorm", "nssm_chunk_scan",
     "nssm_sizeof_scan_args", "nssm_set_wait_polls", "nssm_test_inject_stuck_copy",
     "nssm_spec_workspace_bytes", "nssm_draft_step", "nssm_verify_step", "nssm_commit_step",
-    "nssm_sizeof_token_args",
+    "nssm_sizeof_token_args", "nssm_delta_step", "nssm_sizeof_delta_step_args",
+    "nssm_delta_scan_workspace_bytes", "nssm_delta_scan", "nssm_sizeof_delta_scan_args",
+    "nssm_sizeof_slot_buffer", "nssm_slot_workspace_bytes", "nssm_slot_copy", "nssm_slot_reorder",
+    "nssm_slot_compact", "nssm_beam_workspace_bytes", "nssm_beam_select", "nssm_sizeof_beam_args",
 )
 
 
@@ -105,6 +109,65 @@ class NssmScanArgs(C.Structure):
     ]
 
 
+class NssmDeltaStepArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("num_slots", C.c_int32), ("nheads", C.c_int32), ("ngroups", C.c_int32),
+        ("headdim", C.c_int32), ("dstate", C.c_int32),
+        ("io_dtype", C.c_int32), ("g_dtype", C.c_int32), ("beta_dtype", C.c_int32), ("out_dtype", C.c_int32),
+        ("pad_slot_id", C.c_int32), ("scale", C.c_float),
+        ("state", C.c_void_p), ("state_stride_s", C.c_int64),
+        ("q", C.c_void_p), ("q_stride_b", C.c_int64), ("q_stride_h", C.c_int64),
+        ("k", C.c_void_p), ("k_stride_b", C.c_int64), ("k_stride_h", C.c_int64),
+        ("v", C.c_void_p), ("v_stride_b", C.c_int64), ("v_stride_h", C.c_int64),
+        ("g", C.c_void_p), ("g_stride_b", C.c_int64), ("g_stride_h", C.c_int64),
+        ("beta", C.c_void_p), ("beta_stride_b", C.c_int64), ("beta_stride_h", C.c_int64),
+        ("state_batch_indices", C.c_void_p),
+        ("out", C.c_void_p), ("out_stride_b", C.c_int64), ("out_stride_h", C.c_int64),
+        ("status", C.c_void_p),
+    ]
+
+
+class NssmDeltaScanArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("seqlen", C.c_int32), ("nheads", C.c_int32), ("ngroups", C.c_int32),
+        ("headdim", C.c_int32), ("dstate", C.c_int32), ("g_dtype", C.c_int32), ("beta_dtype", C.c_int32),
+        ("scale", C.c_float), ("_pad0", C.c_int32),
+        ("q", C.c_void_p), ("q_stride_b", C.c_int64), ("q_stride_t", C.c_int64),
+        ("k", C.c_void_p), ("k_stride_b", C.c_int64), ("k_stride_t", C.c_int64),
+        ("v", C.c_void_p), ("v_stride_b", C.c_int64), ("v_stride_t", C.c_int64),
+        ("g", C.c_void_p), ("g_stride_b", C.c_int64), ("g_stride_t", C.c_int64),
+        ("beta", C.c_void_p), ("beta_stride_b", C.c_int64), ("beta_stride_t", C.c_int64),
+        ("cu_seqlens", C.c_void_p),
+        ("initial_states", C.c_void_p), ("init_stride_b", C.c_int64),
+        ("y", C.c_void_p), ("y_stride_b", C.c_int64), ("y_stride_t", C.c_int64),
+        ("final_states", C.c_void_p), ("final_stride_b", C.c_int64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("status", C.c_void_p),
+    ]
+
+
+class NssmSlotBuffer(C.Structure):
+    _fields_ = [
+        ("base", C.c_void_p), ("outer_stride", C.c_int64), ("slot_stride", C.c_int64), ("row_bytes", C.c_int64),
+        ("outer", C.c_int32), ("_pad0", C.c_int32),
+    ]
+
+
+class NssmBeamArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("beams", C.c_int32), ("vocab", C.c_int32), ("nout", C.c_int32),
+        ("logits_dtype", C.c_int32), ("eos_token", C.c_int32),
+        ("logits", C.c_void_p), ("logits_stride_b", C.c_int64), ("logits_stride_k", C.c_int64),
+        ("scores", C.c_void_p), ("finished", C.c_void_p),
+        ("out_scores", C.c_void_p), ("out_parents", C.c_void_p), ("out_tokens", C.c_void_p),
+        ("out_finished", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+MAX_SLOT_BUFFERS, MAX_SLOT_ROWS, MAX_MOVE_SLOTS = 24, 4096, 131072
+MAX_BEAMS, MAX_BEAM_OUT = 64, 128
+
 _lib = None
 _lock = threading.Lock()
 
@@ -159,6 +222,19 @@ def load(auto_build: bool = True) -> C.CDLL:
             "nssm_verify_step": (C.c_int, [P_pool, P_args, C.POINTER(NssmTokenArgs), vp]),
             "nssm_commit_step": (C.c_int, [P_pool, P_args, C.POINTER(NssmTokenArgs), vp]),
             "nssm_sizeof_token_args": (sz, []),
+            "nssm_delta_step": (C.c_int, [C.POINTER(NssmDeltaStepArgs), vp]),
+            "nssm_sizeof_delta_step_args": (sz, []),
+            "nssm_delta_scan_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
+            "nssm_delta_scan": (C.c_int, [C.POINTER(NssmDeltaScanArgs), vp]),
+            "nssm_sizeof_delta_scan_args": (sz, []),
+            "nssm_sizeof_slot_buffer": (sz, []),
+            "nssm_slot_workspace_bytes": (sz, [i32]),
+            "nssm_slot_copy": (C.c_int, [vp, i32, i32, vp, vp, i32, i32, vp, sz, vp, vp]),
+            "nssm_slot_reorder": (C.c_int, [vp, i32, i32, vp, vp, i32, i32, i32, vp, vp, sz, vp, vp]),
+            "nssm_slot_compact": (C.c_int, [vp, i32, i32, vp, i32, i32, vp, vp, sz, vp, vp]),
+            "nssm_beam_workspace_bytes": (sz, [i32, i32, i32, i32, i32]),
+            "nssm_beam_select": (C.c_int, [C.POINTER(NssmBeamArgs), vp]),
+            "nssm_sizeof_beam_args": (sz, []),
         }
         for name, (res, args) in sig.items():
             fn = getattr(lib, name)
@@ -168,7 +244,11 @@ def load(auto_build: bool = True) -> C.CDLL:
         if (lib.nssm_sizeof_pool() != C.sizeof(NssmPool) or lib.nssm_sizeof_step_args() != C.sizeof(NssmStepArgs)
                 or lib.nssm_sizeof_conv_args() != C.sizeof(NssmConvArgs)
                 or lib.nssm_sizeof_scan_args() != C.sizeof(NssmScanArgs)
-                or lib.nssm_sizeof_token_args() != C.sizeof(NssmTokenArgs)):
+                or lib.nssm_sizeof_token_args() != C.sizeof(NssmTokenArgs)
+                or lib.nssm_sizeof_delta_step_args() != C.sizeof(NssmDeltaStepArgs)
+                or lib.nssm_sizeof_delta_scan_args() != C.sizeof(NssmDeltaScanArgs)
+                or lib.nssm_sizeof_slot_buffer() != C.sizeof(NssmSlotBuffer)
+                or lib.nssm_sizeof_beam_args() != C.sizeof(NssmBeamArgs)):
             raise RuntimeError("libnested_ssm struct layout differs from the ctypes binding")
         _lib = lib
         return lib

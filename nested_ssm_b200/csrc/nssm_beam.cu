@@ -1,0 +1,362 @@
+// Beam search's selection: one pass over the logits (sum of exponentials and the nout best of
+// each vocabulary segment), then a merge per prompt.  Bound by HBM: the logits are read once.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "nested_ssm.h"
+
+namespace nssm_host {
+int fail(int code, const char* fmt, ...);
+}
+
+namespace nssm {
+
+constexpr int kBeamThreads = 256;
+constexpr int kVecs = 4;                 // 16-byte pieces of a segment per thread
+constexpr int kMaxOut = NSSM_MAX_BEAM_OUT;
+constexpr float kNegInf = -INFINITY;
+
+struct BeamParams {
+  int b, K, V, n, splits, bf16, eos;
+  const void* logits;
+  int64_t l_b, l_k;
+  const float* scores;
+  const uint8_t* fin;
+  float* out_s;
+  int32_t* out_p;
+  int32_t* out_t;
+  uint8_t* out_f;
+  float2* part;        // [b*K][splits]: max and sum of exp(x - max)
+  uint64_t* cand;      // [b*K][splits][n]: keys, descending; 0 = none
+};
+
+// Candidates order by (logit, lower token): an order-preserving 32-bit image of the logit
+// above the complement of the token.  -inf maps to 0x007fffff, so a key of a real candidate is
+// never 0.
+__device__ __forceinline__ uint32_t order32(float x) {
+  const uint32_t u = __float_as_uint(x + 0.0f);   // -0 and 0 are equal
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float unorder32(uint32_t o) {
+  return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+}
+__device__ __forceinline__ uint64_t key_of(float x, int token) {
+  return ((uint64_t)order32(x) << 32) | (uint32_t)~token;
+}
+__device__ __forceinline__ float masked(float x) { return isfinite(x) ? x : kNegInf; }
+
+// The nth (1-based) largest of kBeamThreads distinct values, by counting for each how many are
+// larger; n <= kBeamThreads.  K: a type with operator<.
+template <typename Key>
+__device__ __forceinline__ Key nth_of_block(Key mine, int n, Key* sh, Key* result) {
+  sh[threadIdx.x] = mine;
+  __syncthreads();
+  int rank = 0;
+  for (int i = 0; i < kBeamThreads; ++i) rank += mine < sh[i];
+  if (rank == n - 1) *result = mine;
+  __syncthreads();
+  return *result;
+}
+
+// Segment of a row: a thread keeps kVecs 16-byte pieces in registers, so the max, the sum and
+// the candidates all come from one read.  A lower bound of the nout-th best candidate is the
+// nout-th largest of the threads' own maxima; only the few candidates above it are ranked.
+template <bool BF16>
+__global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const BeamParams p) {
+  constexpr int E = BF16 ? 8 : 4;                       // elements of a 16-byte piece
+  constexpr int kSeg = kBeamThreads * kVecs * E;
+  constexpr int kCap = kMaxOut * kVecs * E;             // candidates of kMaxOut threads
+  __shared__ uint64_t sh[kBeamThreads];
+  __shared__ uint64_t list[kCap];
+  __shared__ float red[kBeamThreads / 32];
+  __shared__ uint64_t nth;
+  __shared__ int count;
+  const int row = blockIdx.y, bi = row / p.K, ki = row - bi * p.K, split = blockIdx.x;
+  if (p.fin && p.fin[row]) return;                      // the merge knows its one candidate
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int es = BF16 ? 2 : 4;
+  const char* base = static_cast<const char*>(p.logits) + (bi * p.l_b + ki * p.l_k) * es;
+  // pieces are 16-byte aligned in memory: piece 0 of the row may begin before the row does
+  const int lead = (int)((reinterpret_cast<uintptr_t>(base) & 15) / es);
+  float x[kVecs * E];
+  int tok0[kVecs];
+  float mx = kNegInf;
+#pragma unroll
+  for (int c = 0; c < kVecs; ++c) {
+    const int t0 = split * kSeg + (c * kBeamThreads + tid) * E - lead;
+    tok0[c] = t0;
+    if (t0 >= 0 && t0 + E <= p.V) {
+      const uint4 r = __ldg(reinterpret_cast<const uint4*>(base + (int64_t)t0 * es));
+      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (BF16) {
+          x[c * E + 2 * i] = __uint_as_float(w[i] << 16);
+          x[c * E + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+          x[c * E + i] = __uint_as_float(w[i]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int t = t0 + i;
+        x[c * E + i] = kNegInf;
+        if (t >= 0 && t < p.V)
+          x[c * E + i] = BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[t])
+                              : reinterpret_cast<const float*>(base)[t];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      x[c * E + i] = masked(x[c * E + i]);
+      mx = fmaxf(mx, x[c * E + i]);
+    }
+  }
+  // the thread's best key (0: no token of the row)
+  uint64_t best = 0;
+#pragma unroll
+  for (int c = 0; c < kVecs; ++c)
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int t = tok0[c] + i;
+      const uint64_t k = (t >= 0 && t < p.V) ? key_of(x[c * E + i], t) : 0;
+      best = k > best ? k : best;
+    }
+  float m = mx;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) red[warp] = m;
+  if (tid == 0) count = 0;
+  __syncthreads();
+  m = red[0];
+#pragma unroll
+  for (int w = 1; w < kBeamThreads / 32; ++w) m = fmaxf(m, red[w]);
+  __syncthreads();
+  float sum = 0.0f;
+  if (m != kNegInf)
+#pragma unroll
+    for (int i = 0; i < kVecs * E; ++i) sum += expf(x[i] - m);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) red[warp] = sum;
+  // threads without a token get distinct keys below every real one (those have bit 63..32 >= 0x007fffff)
+  const uint64_t tau = nth_of_block<uint64_t>(best ? best : (uint64_t)tid, p.n, sh, &nth);
+  if (tid == 0) {
+    float s = 0.0f;
+    for (int w = 0; w < kBeamThreads / 32; ++w) s += red[w];
+    p.part[(int64_t)row * p.splits + split] = make_float2(m, s);
+  }
+  if (best && best >= tau)
+#pragma unroll
+    for (int c = 0; c < kVecs; ++c)
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int t = tok0[c] + i;
+        if (t < 0 || t >= p.V) continue;
+        const uint64_t k = key_of(x[c * E + i], t);
+        if (k >= tau) list[atomicAdd(&count, 1)] = k;
+      }
+  __syncthreads();
+  const int cnt = count;
+  uint64_t* out = p.cand + ((int64_t)row * p.splits + split) * p.n;
+  for (int i = tid; i < p.n; i += kBeamThreads)
+    if (i >= cnt) out[i] = 0;
+  for (int i = tid; i < cnt; i += kBeamThreads) {
+    const uint64_t k = list[i];
+    int rank = 0;
+    for (int j = 0; j < cnt; ++j) rank += list[j] > k;
+    if (rank < p.n) out[rank] = k;
+  }
+}
+
+// A candidate of the merge: its total, then the lower beam, then the beam's own order.
+struct BeamKey {
+  uint64_t hi;         // order-preserving image of the 64-bit total; 0 = none
+  uint64_t lo;         // complement of the beam, logit order, complement of the token
+  __device__ __forceinline__ bool operator<(const BeamKey& o) const { return hi < o.hi || (hi == o.hi && lo < o.lo); }
+};
+__device__ __forceinline__ uint64_t order64(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);
+  return (u >> 63) ? ~u : (u | (1ull << 63));
+}
+__device__ __forceinline__ double unorder64(uint64_t o) {
+  return __longlong_as_double((long long)((o >> 63) ? (o & ~(1ull << 63)) : ~o));
+}
+
+constexpr int kBlock = 4 * kBeamThreads;     // candidates looked at together
+constexpr int kBeamBits = 6, kTokenBits = 26;
+static_assert(NSSM_MAX_BEAMS <= 1 << kBeamBits && kBeamBits + kTokenBits == 32, "fields of BeamKey::lo");
+
+// One prompt: the nout best of all candidates.  The segments' lists are sorted, so candidates
+// come in the order of their rank: the first block holds the heads of the lists, and once no list
+// has anything above the nout-th best so far at some rank, nothing behind it has.
+__global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamParams p) {
+  __shared__ double lse[NSSM_MAX_BEAMS];
+  __shared__ BeamKey sh[kBeamThreads];
+  __shared__ BeamKey cur[kMaxOut], list[kBlock + kMaxOut];
+  __shared__ BeamKey nth;
+  __shared__ int count;
+  const int bi = blockIdx.x, tid = threadIdx.x;
+  for (int k = tid >> 5; k < p.K; k += kBeamThreads / 32) {   // a warp per beam
+    const int64_t row = (int64_t)bi * p.K + k;
+    const bool fin = p.fin && p.fin[row];
+    float m = kNegInf;
+    if (!fin)
+      for (int s = tid & 31; s < p.splits; s += 32) m = fmaxf(m, p.part[row * p.splits + s].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    double sum = 0.0;
+    if (!fin && m != kNegInf)
+      for (int s = tid & 31; s < p.splits; s += 32) {
+        const float2 q = p.part[row * p.splits + s];
+        if (q.x != kNegInf) sum += (double)q.y * exp((double)q.x - (double)m);
+      }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((tid & 31) == 0) lse[k] = fin ? 0.0 : m == kNegInf ? (double)kNegInf : log(sum) + (double)m;
+  }
+  __syncthreads();
+  const int lists = p.K * p.splits, per = min(p.n, p.V);
+  const int64_t all = (int64_t)lists * per;
+  int have = 0, quiet = 0;   // entries of cur; candidates since the last one that counted
+  for (int64_t c0 = 0; c0 < all && quiet < lists; c0 += kBlock) {
+    BeamKey key[4], best{0, (uint64_t)tid};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      key[u] = BeamKey{0, 0};
+      const int64_t c = c0 + u * kBeamThreads + tid;
+      if (c >= all) continue;
+      const int j = (int)(c / lists), l = (int)(c - (int64_t)j * lists), k = l / p.splits, split = l - k * p.splits;
+      const int64_t row = (int64_t)bi * p.K + k;
+      float x;
+      uint32_t tok;
+      if (p.fin && p.fin[row]) {
+        if (split) continue;
+        tok = j == 0 ? p.eos : j - 1 < p.eos ? j - 1 : j;
+        x = j == 0 ? 0.0f : kNegInf;
+      } else {
+        const uint64_t q = p.cand[(row * p.splits + split) * p.n + j];
+        if (!q) continue;
+        tok = ~(uint32_t)q;
+        x = unorder32((uint32_t)(q >> 32));
+      }
+      double total = ((double)p.scores[row] + (double)x) - lse[k];
+      if (isnan(total)) total = (double)kNegInf;
+      key[u].hi = order64(total);
+      key[u].lo = ((uint64_t)((1 << kBeamBits) - 1 - k) << (32 + kTokenBits)) | ((uint64_t)order32(x) << kTokenBits) |
+                  (~tok & ((1u << kTokenBits) - 1));
+      if (best < key[u]) best = key[u];
+    }
+    if (tid == 0) count = 0;
+    BeamKey tau;
+    if (c0 == 0)
+      tau = nth_of_block<BeamKey>(best, p.n, sh, &nth);
+    else
+      tau = have == p.n ? cur[p.n - 1] : BeamKey{0, 0};
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (key[u].hi && !(key[u] < tau)) list[atomicAdd(&count, 1)] = key[u];
+    __syncthreads();
+    const int found = count;
+    if (found) {
+      quiet = 0;
+      for (int i = tid; i < have; i += kBeamThreads) list[found + i] = cur[i];
+      __syncthreads();
+      const int m = found + have;
+      for (int i = tid; i < m; i += kBeamThreads) {
+        const BeamKey k = list[i];
+        int rank = 0;
+        for (int j = 0; j < m; ++j) rank += k < list[j];
+        if (rank < p.n) cur[rank] = k;
+      }
+      have = min(m, p.n);
+    } else {
+      quiet += kBlock;
+    }
+    __syncthreads();
+  }
+  for (int i = tid; i < p.n; i += kBeamThreads) {
+    const BeamKey k = cur[i];
+    const int beam = (1 << kBeamBits) - 1 - (int)(k.lo >> (32 + kTokenBits));
+    const int tok = (int)(~(uint32_t)k.lo & ((1u << kTokenBits) - 1));
+    const int64_t o = (int64_t)bi * p.n + i;
+    p.out_s[o] = (float)unorder64(k.hi);
+    p.out_p[o] = beam;
+    p.out_t[o] = tok;
+    if (p.out_f) p.out_f[o] = (tok == p.eos) || (p.fin && p.fin[(int64_t)bi * p.K + beam]);
+  }
+}
+
+}  // namespace nssm
+
+namespace {
+
+using nssm_host::fail;
+
+int segments(int V, int bf16) {
+  const int seg = nssm::kBeamThreads * nssm::kVecs * (bf16 ? 8 : 4);
+  return (int)(((int64_t)V + (bf16 ? 7 : 3) + seg - 1) / seg);   // a row may begin inside its first piece
+}
+size_t part_bytes(int64_t rows, int splits) { return ((size_t)rows * splits * sizeof(float2) + 255) / 256 * 256; }
+
+}  // namespace
+
+extern "C" {
+
+size_t nssm_sizeof_beam_args(void) { return sizeof(nssm_beam_args); }
+
+size_t nssm_beam_workspace_bytes(int32_t batch, int32_t beams, int32_t vocab, int32_t nout, int32_t logits_dtype) {
+  if (batch <= 0 || beams <= 0 || vocab <= 0 || nout <= 0) return 0;
+  const int splits = segments(vocab, logits_dtype == NSSM_BF16);
+  const int64_t rows = (int64_t)batch * beams;
+  return part_bytes(rows, splits) + (size_t)rows * splits * nout * sizeof(uint64_t);
+}
+
+int nssm_beam_select(const nssm_beam_args* a, void* stream) {
+  if (!a) return fail(NSSM_ERR_INVALID, "args is NULL");
+  if (a->batch < 0 || a->beams <= 0 || a->beams > NSSM_MAX_BEAMS)
+    return fail(NSSM_ERR_INVALID, "batch %d, beams %d (1 to %d)", a->batch, a->beams, NSSM_MAX_BEAMS);
+  if (a->vocab <= 0 || a->vocab > (1 << nssm::kTokenBits))
+    return fail(NSSM_ERR_INVALID, "vocab %d outside [1, %d]", a->vocab, 1 << nssm::kTokenBits);
+  if (a->nout <= 0 || a->nout > NSSM_MAX_BEAM_OUT || a->nout > (int64_t)a->beams * a->vocab)
+    return fail(NSSM_ERR_INVALID, "nout %d outside [1, min(%d, beams * vocab)]", a->nout, NSSM_MAX_BEAM_OUT);
+  if (a->logits_dtype != NSSM_F32 && a->logits_dtype != NSSM_BF16)
+    return fail(NSSM_ERR_INVALID, "logits dtype must be F32 or BF16");
+  if (a->eos_token >= a->vocab) return fail(NSSM_ERR_INVALID, "eos_token %d outside the vocabulary", a->eos_token);
+  if (a->finished && a->eos_token < 0) return fail(NSSM_ERR_INVALID, "finished beams need an eos_token");
+  const int64_t rows = (int64_t)a->batch * a->beams;
+  if (rows > 65535) return fail(NSSM_ERR_INVALID, "batch * beams %lld beyond 65535", (long long)rows);
+  if (a->batch == 0) return NSSM_OK;
+  if (!a->logits || !a->scores || !a->out_scores || !a->out_parents || !a->out_tokens)
+    return fail(NSSM_ERR_INVALID, "logits/scores/outputs must be non-NULL");
+  const size_t need = nssm_beam_workspace_bytes(a->batch, a->beams, a->vocab, a->nout, a->logits_dtype);
+  if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 15) || a->workspace_bytes < need)
+    return fail(NSSM_ERR_INVALID, "a 16-byte aligned workspace of %zu bytes is needed (got %zu)", need, a->workspace_bytes);
+  nssm::BeamParams p{};
+  p.b = a->batch; p.K = a->beams; p.V = a->vocab; p.n = a->nout; p.eos = a->eos_token;
+  p.bf16 = a->logits_dtype == NSSM_BF16;
+  p.splits = segments(p.V, p.bf16);
+  p.logits = a->logits; p.l_b = a->logits_stride_b; p.l_k = a->logits_stride_k;
+  p.scores = a->scores; p.fin = a->finished;
+  p.out_s = a->out_scores; p.out_p = a->out_parents; p.out_t = a->out_tokens; p.out_f = a->out_finished;
+  p.part = static_cast<float2*>(a->workspace);
+  p.cand = reinterpret_cast<uint64_t*>(static_cast<char*>(a->workspace) + part_bytes(rows, p.splits));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const dim3 grid(p.splits, (unsigned)rows);
+  if (p.bf16)
+    nssm::beam_scan_kernel<true><<<grid, nssm::kBeamThreads, 0, st>>>(p);
+  else
+    nssm::beam_scan_kernel<false><<<grid, nssm::kBeamThreads, 0, st>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(NSSM_ERR_CUDA, "beam_scan_kernel launch: %s", cudaGetErrorString(e));
+  nssm::beam_merge_kernel<<<p.b, nssm::kBeamThreads, 0, st>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(NSSM_ERR_CUDA, "beam_merge_kernel launch: %s", cudaGetErrorString(e));
+  return NSSM_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,234 @@
+// The gated delta rule on states S[headdim][dstate] (fp32), per value head h:
+//   S <- e^g S;  u = beta (v - S k);  S <- S + u k^T;  y = scale S q
+// Decode (delta_step_kernel) and prompts token by token (delta_scan_kernel).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "nested_ssm.h"
+
+namespace nssm {
+
+enum : int { STATUS_CONFLICT = NSSM_STATUS_CONFLICT };
+
+struct DeltaStepParams {
+  int H, G, P, S, ns, rows;   // ns slices of `rows` headdim rows per head
+  int pad;
+  int io_bf16, g_bf16, beta_bf16, out_bf16;
+  int vec;                    // q and k rows are 8-byte (bf16) / 16-byte (fp32) aligned
+  float scale;
+  float* state;
+  int64_t st_s;
+  const void *q, *k, *v, *g, *beta;
+  int64_t q_b, q_h, k_b, k_h, v_b, v_h, g_b, g_h, beta_b, beta_h;
+  const int32_t* idx;
+  void* out;
+  int64_t o_b, o_h;
+  int32_t* status;
+};
+
+__device__ __forceinline__ float dl_ld(const void* p, int64_t i, int bf16) {
+  return bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]) : reinterpret_cast<const float*>(p)[i];
+}
+__device__ __forceinline__ void dl_st(void* p, int64_t i, int bf16, float v) {
+  if (bf16)
+    reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else
+    reinterpret_cast<float*>(p)[i] = v;
+}
+__device__ __forceinline__ float4 dl_ld4(const void* p, int64_t i, int bf16, int vec) {
+  if (vec) {
+    if (bf16) {
+      const uint2 r = *reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(p) + i);
+      return make_float4(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u), __uint_as_float(r.y << 16),
+                         __uint_as_float(r.y & 0xffff0000u));
+    }
+    return *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
+  }
+  return make_float4(dl_ld(p, i, bf16), dl_ld(p, i + 1, bf16), dl_ld(p, i + 2, bf16), dl_ld(p, i + 3, bf16));
+}
+__device__ __forceinline__ float dot4(float4 a, float4 b, float acc) {
+  return fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, acc))));
+}
+// sum over the 8 lanes that share a state row
+__device__ __forceinline__ float sum8(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  v += __shfl_xor_sync(0xffffffffu, v, 2);
+  return v + __shfl_xor_sync(0xffffffffu, v, 4);
+}
+
+// One decode token.  A CTA takes `rows` state rows of one (batch row, head); 8 lanes share a state
+// row, each with N/32 16-byte pieces of it, so both dot products of a row reduce in 3 shuffles.
+// The output is read off the old state, y = scale (e^g S q + u (k.q)), so that S k and S q reduce
+// together and the row is touched once.
+template <int N>
+__global__ void __launch_bounds__(320) delta_step_kernel(const DeltaStepParams p) {
+  constexpr int V = N / 32;
+  const int b = blockIdx.y, h = blockIdx.x / p.ns, slice = blockIdx.x - h * p.ns;
+  const int tid = threadIdx.x, l8 = tid & 7;
+  const int r = slice * p.rows + (tid >> 3);
+  const int slot = p.idx ? p.idx[b] : b;
+  if (slot == p.pad) return;
+  if (slot < 0 || slot >= p.S) {
+    if (p.status && blockIdx.x == 0 && tid == 0) atomicOr(p.status, 1);
+    return;
+  }
+  const bool live = r < p.P;
+  float* row = p.state + (int64_t)slot * p.st_s + ((int64_t)h * p.P + (live ? r : 0)) * N;
+  float4 s[V], kk[V], qq[V];
+#pragma unroll
+  for (int c = 0; c < V; ++c) s[c] = reinterpret_cast<const float4*>(row)[l8 + 8 * c];
+  // the first row that names a slot owns it
+  int dup = 0;
+  if (p.idx)
+    for (int i = tid; i < b; i += blockDim.x) dup |= p.idx[i] == slot;
+  const int kh = h / (p.H / p.G);
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    const int n = 4 * (l8 + 8 * c);
+    kk[c] = dl_ld4(p.k, b * p.k_b + kh * p.k_h + n, p.io_bf16, p.vec);
+    qq[c] = dl_ld4(p.q, b * p.q_b + kh * p.q_h + n, p.io_bf16, p.vec);
+  }
+  const float eg = expf(dl_ld(p.g, b * p.g_b + h * p.g_h, p.g_bf16));
+  const float beta = dl_ld(p.beta, b * p.beta_b + h * p.beta_h, p.beta_bf16);
+  const float v = live ? dl_ld(p.v, b * p.v_b + h * p.v_h + r, p.io_bf16) : 0.0f;
+  float sk = 0.0f, sq = 0.0f, kq = 0.0f;
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    s[c].x *= eg; s[c].y *= eg; s[c].z *= eg; s[c].w *= eg;
+    sk = dot4(s[c], kk[c], sk);
+    sq = dot4(s[c], qq[c], sq);
+    kq = dot4(kk[c], qq[c], kq);
+  }
+  sk = sum8(sk); sq = sum8(sq); kq = sum8(kq);
+  const float u = beta * (v - sk);
+  if (__syncthreads_or(dup)) {
+    if (p.status && blockIdx.x == 0 && tid == 0) atomicOr(p.status, STATUS_CONFLICT);
+    return;
+  }
+  if (!live) return;
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    s[c].x = fmaf(u, kk[c].x, s[c].x); s[c].y = fmaf(u, kk[c].y, s[c].y);
+    s[c].z = fmaf(u, kk[c].z, s[c].z); s[c].w = fmaf(u, kk[c].w, s[c].w);
+    reinterpret_cast<float4*>(row)[l8 + 8 * c] = s[c];
+  }
+  if (l8 == 0) dl_st(p.out, b * p.o_b + h * p.o_h + r, p.out_bf16, p.scale * fmaf(u, kq, sq));
+}
+
+struct DeltaScanParams {
+  int B, T, H, G, P, ns, rows;
+  int g_bf16, beta_bf16;
+  float scale;
+  const __nv_bfloat16 *q, *k, *v;
+  int64_t q_b, q_t, k_b, k_t, v_b, v_t;
+  const void *g, *beta;
+  int64_t g_b, g_t, beta_b, beta_t;
+  const int32_t* cu;
+  const float* init;
+  int64_t init_b;
+  __nv_bfloat16* y;
+  int64_t y_b, y_t;
+  float* fin;
+  int64_t fin_b;
+  int32_t* status;
+};
+
+// Tokens [t0, t0 + len) of sequence s (in its own batch row, or packed); false: bad bounds.
+__device__ __forceinline__ bool delta_seq(const DeltaScanParams& p, int s, int* batch, int* t0, int* len) {
+  if (!p.cu) {
+    *batch = s; *t0 = 0; *len = p.T;
+    return true;
+  }
+  const int a = p.cu[s], e = p.cu[s + 1];
+  *batch = 0; *t0 = a; *len = e - a;
+  return a >= 0 && e >= a && e <= p.T;
+}
+
+constexpr int kScanTok = 16;   // tokens staged at a time
+
+// A prompt token by token, the state in registers (the layout of delta_step_kernel); q and k of
+// kScanTok tokens are staged as fp32 in shared memory.
+template <int N>
+__global__ void __launch_bounds__(320) delta_scan_kernel(const DeltaScanParams p) {
+  constexpr int V = N / 32;
+  __shared__ float sq[kScanTok][N], sk[kScanTok][N];
+  __shared__ float sv[kScanTok][40], sg[kScanTok], sb[kScanTok], skq[kScanTok];
+  const int s = blockIdx.y, h = blockIdx.x / p.ns, slice = blockIdx.x - h * p.ns;
+  const int tid = threadIdx.x, l8 = tid & 7, rl = tid >> 3;
+  const int r = slice * p.rows + rl;
+  const bool live = r < p.P;
+  int batch, t0, len;
+  if (!delta_seq(p, s, &batch, &t0, &len)) {
+    if (p.status && blockIdx.x == 0 && tid == 0) atomicOr(p.status, STATUS_CONFLICT);
+    return;
+  }
+  const int64_t off = ((int64_t)h * p.P + (live ? r : 0)) * N;
+  float4 st[V];
+#pragma unroll
+  for (int c = 0; c < V; ++c)
+    st[c] = p.init ? reinterpret_cast<const float4*>(p.init + s * p.init_b + off)[l8 + 8 * c]
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
+  const int kh = h / (p.H / p.G);
+  for (int tb = 0; tb < len; tb += kScanTok) {
+    const int nt = min(kScanTok, len - tb);
+    __syncthreads();
+    for (int i = tid; i < nt * (N / 2); i += blockDim.x) {
+      const int t = i / (N / 2), n = 2 * (i - t * (N / 2));
+      const int64_t tok = t0 + tb + t;
+      const float2 fk = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p.k + batch * p.k_b + tok * p.k_t + kh * N + n));
+      const float2 fq = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p.q + batch * p.q_b + tok * p.q_t + kh * N + n));
+      sk[t][n] = fk.x; sk[t][n + 1] = fk.y;
+      sq[t][n] = fq.x; sq[t][n + 1] = fq.y;
+    }
+    for (int i = tid; i < nt * p.rows; i += blockDim.x) {
+      const int t = i / p.rows, c = i - t * p.rows;
+      const int64_t tok = t0 + tb + t;
+      sv[t][c] = slice * p.rows + c < p.P ? __bfloat162float(p.v[batch * p.v_b + tok * p.v_t + h * p.P + slice * p.rows + c]) : 0.0f;
+    }
+    if (tid < nt) {
+      const int64_t tok = t0 + tb + tid;
+      sg[tid] = expf(dl_ld(p.g, batch * p.g_b + tok * p.g_t + h, p.g_bf16));
+      sb[tid] = dl_ld(p.beta, batch * p.beta_b + tok * p.beta_t + h, p.beta_bf16);
+    }
+    __syncthreads();
+    for (int t = tid >> 5; t < nt; t += blockDim.x >> 5) {   // k.q of each token, one warp each
+      float a = 0.0f;
+      for (int n = tid & 31; n < N; n += 32) a = fmaf(sk[t][n], sq[t][n], a);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+      if ((tid & 31) == 0) skq[t] = a;
+    }
+    __syncthreads();
+    for (int t = 0; t < nt; ++t) {
+      float a = 0.0f, c2 = 0.0f;
+      const float eg = sg[t];
+      float4 kk[V];
+#pragma unroll
+      for (int c = 0; c < V; ++c) {
+        kk[c] = reinterpret_cast<const float4*>(sk[t])[l8 + 8 * c];
+        const float4 qq = reinterpret_cast<const float4*>(sq[t])[l8 + 8 * c];
+        st[c].x *= eg; st[c].y *= eg; st[c].z *= eg; st[c].w *= eg;
+        a = dot4(st[c], kk[c], a);
+        c2 = dot4(st[c], qq, c2);
+      }
+      a = sum8(a); c2 = sum8(c2);
+      const float u = sb[t] * (sv[t][rl] - a);
+#pragma unroll
+      for (int c = 0; c < V; ++c) {
+        st[c].x = fmaf(u, kk[c].x, st[c].x); st[c].y = fmaf(u, kk[c].y, st[c].y);
+        st[c].z = fmaf(u, kk[c].z, st[c].z); st[c].w = fmaf(u, kk[c].w, st[c].w);
+      }
+      if (l8 == 0 && live)
+        p.y[batch * p.y_b + (int64_t)(t0 + tb + t) * p.y_t + h * p.P + r] =
+            __float2bfloat16_rn(p.scale * fmaf(u, skq[t], c2));
+    }
+  }
+  if (p.fin && live)
+#pragma unroll
+    for (int c = 0; c < V; ++c) reinterpret_cast<float4*>(p.fin + s * p.fin_b + off)[l8 + 8 * c] = st[c];
+}
+
+}  // namespace nssm

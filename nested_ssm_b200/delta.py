@@ -1,0 +1,177 @@
+"""The gated delta rule: a recurrent state rule beside the Mamba2 update, on states of the same
+layout ``[slot, H, P, N]`` (fp32).  Per value head, with the log decay ``g`` and the write strength
+``beta``:
+
+    S <- exp(g) S;   u = beta (v - S k);   S <- S + u k^T;   y = scale S q
+
+* :func:`gated_delta_state_update` -- one decode token per row with continuous-batching
+  ``state_batch_indices``, beside :func:`~nested_ssm_b200.ops.selective_state_update`.
+* :func:`gated_delta_chunk_scan` -- prompts (padded or packed), beside
+  :func:`~nested_ssm_b200.ops.mamba_chunk_scan_combined`.
+
+Inference only: tensors that require a gradient are refused.  All tensors must live on the same
+CUDA device; work is enqueued on that device's current stream and never synchronised.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+from .ops import _ptr, _require_cuda, _stream
+from .pool import nssm_dtype
+
+_IO = (torch.bfloat16, torch.float32)
+
+
+def _no_grad(*ts):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError("no backward pass: call under torch.no_grad() or detach the inputs")
+
+
+def _check_status(status):
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
+        raise ValueError("status must be an int32 tensor")
+
+
+def _indices(idx, n, name):
+    idx = idx.reshape(-1)
+    if idx.numel() != n:
+        raise ValueError(f"{name} has {idx.numel()} entries, expected {n}")
+    if idx.dtype != torch.int32 or not idx.is_contiguous():
+        idx = idx.to(torch.int32).contiguous()
+    return idx
+
+
+def gated_delta_state_update(state: torch.Tensor, q, k, v, g, beta, scale: float | None = None,
+                             state_batch_indices=None, pad_slot_id: int = -1, out=None, status=None):
+    """One decode token of the gated delta rule on ``state [S, H, P, N]`` (fp32, updated in
+    place; heads packed, slots at any stride that is a multiple of 4); returns ``out [b, H, P]``.
+
+    ``q``, ``k`` ``[b, G, N]`` and ``v`` ``[b, H, P]`` bf16 or fp32 (head h uses group
+    ``h // (H // G)``); ``g`` (log decay), ``beta`` ``[b, H]`` bf16 or fp32; ``scale`` defaults to
+    ``N ** -0.5``.  Compiled for N 64 and 128, P a multiple of 16 up to 256.  Row b works on slot
+    ``state_batch_indices[b]`` (row b without them); rows whose slot is ``pad_slot_id`` are skipped
+    and their ``out`` rows untouched, as are rows whose slot is out of range (bit 0 of the int32
+    ``status``) or was named by an earlier row (bit 3)."""
+    if state.dim() != 4 or state.dtype != torch.float32:
+        raise ValueError(f"state must be an fp32 [S, H, P, N] tensor, got {tuple(state.shape)} {state.dtype}")
+    S, H, P, N = state.shape
+    if state.stride()[1:] != (P * N, N, 1):
+        raise ValueError("the heads of a slot must be contiguous in state")
+    if q.dim() != 3 or k.shape != q.shape or q.shape[2] != N:
+        raise ValueError(f"q and k must be [b, G, {N}], got {tuple(q.shape)} and {tuple(k.shape)}")
+    b, G = q.shape[:2]
+    if v.shape != (b, H, P) or g.shape != (b, H) or beta.shape != (b, H):
+        raise ValueError(f"v must be [{b}, {H}, {P}], g and beta [{b}, {H}], got {tuple(v.shape)}, {tuple(g.shape)}, "
+                         f"{tuple(beta.shape)}")
+    if q.dtype not in _IO or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must share a bf16 / fp32 dtype")
+    _no_grad(state, q, k, v, g, beta)
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    if k.stride(2) != 1:
+        k = k.contiguous()
+    if v.stride(2) != 1:
+        v = v.contiguous()
+    idx = None if state_batch_indices is None else _indices(state_batch_indices, b, "state_batch_indices")
+    _check_status(status)
+    if out is None:
+        out = torch.empty(b, H, P, dtype=q.dtype, device=state.device)
+    elif out.shape != (b, H, P) or out.stride(2) != 1 or out.dtype not in _IO:
+        raise ValueError(f"out must be [{b}, {H}, {P}] bf16 / fp32 with unit inner stride")
+    dev = _require_cuda(state, q, k, v, g, beta, idx, out, status)
+    a = _lib.NssmDeltaStepArgs(
+        b, S, H, G, P, N, nssm_dtype(q.dtype), nssm_dtype(g.dtype), nssm_dtype(beta.dtype), nssm_dtype(out.dtype),
+        int(pad_slot_id), N ** -0.5 if scale is None else float(scale),
+        state.data_ptr(), state.stride(0), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
+        k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), g.data_ptr(), g.stride(0), g.stride(1),
+        beta.data_ptr(), beta.stride(0), beta.stride(1), _ptr(idx), out.data_ptr(), out.stride(0), out.stride(1),
+        _ptr(status))
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        _lib.check(lib.nssm_delta_step(C.byref(a), _stream(dev)))
+    return out
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``[b, T, heads, dim]`` with packed (heads, dim), 16-byte aligned tokens and no broadcast
+    axis: what the kernel loads; copied when it is not so."""
+    b, T, h, d = t.shape
+    s = t.stride()
+    if s[3] != 1 or s[2] != d or s[1] % 8 or s[0] % 8 or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.data_ptr() % 16:     # a contiguous view that begins inside a 16-byte piece
+            t = t.clone()
+    return t
+
+
+def gated_delta_chunk_scan(q, k, v, g, beta, scale: float | None = None, initial_states=None, cu_seqlens=None,
+                           return_final_states: bool = False, *, out=None, final_states=None, status=None):
+    """The gated delta rule over prompts: ``q``, ``k`` ``[b, T, G, N]`` and ``v`` ``[b, T, H, P]``
+    bf16, ``g`` (log decay) and ``beta`` ``[b, T, H]`` bf16 or fp32; returns ``y [b, T, H, P]``
+    (bf16) and with ``return_final_states`` also the fp32 states ``[n, H, P, N]`` after the last
+    token of each sequence.  ``scale`` defaults to ``N ** -0.5``; N 64 or 128, P a multiple of 16 up
+    to 256.
+
+    ``cu_seqlens`` (int32 ``[n + 1]`` on the device, b == 1): sequence s has the tokens
+    ``cu_seqlens[s]`` to ``cu_seqlens[s + 1]``; empty sequences keep their initial state, and
+    the rows of ``out`` outside every sequence are left as they were.  Sequences whose bounds
+    do not ascend inside ``[0, T]`` are skipped and set bit 3 of the int32 ``status``.  Otherwise
+    n == b.  ``initial_states [n, H, P, N]`` fp32 (zeros without them); ``final_states`` may be the
+    same tensor.  ``g`` may be ``-inf`` (the state is forgotten)."""
+    if q.dim() != 4 or k.shape != q.shape or v.dim() != 4 or g.dim() != 3 or beta.dim() != 3:
+        raise ValueError("q / k [b, T, G, N], v [b, T, H, P], g / beta [b, T, H] expected")
+    b, T, G, N = q.shape
+    H, P = v.shape[2:]
+    if v.shape[:2] != (b, T) or g.shape != (b, T, H) or beta.shape != (b, T, H):
+        raise ValueError(f"shape mismatch: q {tuple(q.shape)} v {tuple(v.shape)} g {tuple(g.shape)} "
+                         f"beta {tuple(beta.shape)}")
+    if q.dtype != torch.bfloat16 or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise ValueError("q, k and v must be bf16")
+    _no_grad(q, k, v, g, beta, initial_states)
+    n = b
+    if cu_seqlens is not None:
+        if b != 1 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+            raise ValueError("cu_seqlens [n + 1] needs packed inputs with b == 1")
+        n = cu_seqlens.numel() - 1
+        cu_seqlens = _indices(cu_seqlens, n + 1, "cu_seqlens")
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    if g.stride(2) != 1:
+        g = g.contiguous()
+    if beta.stride(2) != 1:
+        beta = beta.contiguous()
+    inner = (P * N, N, 1)
+    if initial_states is not None:
+        if initial_states.shape != (n, H, P, N):
+            raise ValueError(f"initial_states must be [{n}, {H}, {P}, {N}], got {tuple(initial_states.shape)}")
+        if (initial_states.dtype != torch.float32 or initial_states.stride()[1:] != inner
+                or initial_states.stride(0) % 4 or initial_states.data_ptr() % 16):
+            initial_states = initial_states.float().contiguous()
+    if out is None:
+        out = torch.empty(b, T, H, P, dtype=torch.bfloat16, device=q.device)
+    elif out.shape != (b, T, H, P) or out.dtype != torch.bfloat16 or out.stride()[2:] != (P, 1):
+        raise ValueError("out must be bf16 [b, T, H, P] with packed (H, P)")
+    if final_states is not None:
+        if (final_states.shape != (n, H, P, N) or final_states.dtype != torch.float32
+                or final_states.stride()[1:] != inner):
+            raise ValueError(f"final_states must be fp32 [{n}, {H}, {P}, {N}] with contiguous rows")
+    elif return_final_states:
+        final_states = torch.empty(n, H, P, N, dtype=torch.float32, device=q.device)
+    _check_status(status)
+    dev = _require_cuda(q, k, v, g, beta, cu_seqlens, initial_states, out, final_states, status)
+    lib = _lib.load()
+    nbytes = lib.nssm_delta_scan_workspace_bytes(n, T, H, P, N, int(cu_seqlens is not None))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    a = _lib.NssmDeltaScanArgs(
+        n, T, H, G, P, N, nssm_dtype(g.dtype), nssm_dtype(beta.dtype), N ** -0.5 if scale is None else float(scale), 0,
+        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+        v.data_ptr(), v.stride(0), v.stride(1), g.data_ptr(), g.stride(0), g.stride(1),
+        beta.data_ptr(), beta.stride(0), beta.stride(1), _ptr(cu_seqlens),
+        _ptr(initial_states), initial_states.stride(0) if initial_states is not None else 0,
+        out.data_ptr(), out.stride(0), out.stride(1),
+        _ptr(final_states), final_states.stride(0) if final_states is not None else 0, _ptr(ws), nbytes, _ptr(status))
+    with torch.cuda.device(dev):
+        _lib.check(lib.nssm_delta_scan(C.byref(a), _stream(dev)))
+    return (out, final_states) if return_final_states else out

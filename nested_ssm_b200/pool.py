@@ -75,6 +75,7 @@ class TieredSlotPool:
         ws = lib.nssm_step_workspace_bytes(self.max_batch, G, dstate, nssm_dtype(io_dtype), 1)
         self.workspace = torch.empty(max(ws, 256), dtype=torch.uint8, device=device)
         self._structs = [self._make_struct(l) for l in range(L)]
+        self._slot_bufs = None    # descriptors of the buffers for slot moves, made at the first one
 
     # ------------------------------------------------------------------
     def _make_struct(self, l: int) -> _lib.NssmPool:
@@ -107,7 +108,8 @@ class TieredSlotPool:
     def check_status(self) -> None:
         """Raise if a kernel flagged an error since the last reset (synchronises): bit 0 a slot
         index outside the pool, bit 1 a pipeline wait that timed out, bit 2 a verify / commit
-        window across a chunk boundary or an accept count out of range."""
+        window across a chunk boundary or an accept count out of range, bit 3 a slot move dropped
+        (a slot named twice, or both read and written)."""
         v = int(self.status.item())
         if v:
             self.status.zero_()
@@ -118,6 +120,8 @@ class TieredSlotPool:
                 what.append("a pipeline wait timed out")
             if v & 4:
                 what.append("a verify / commit window crosses a chunk boundary or accept is out of range")
+            if v & _lib.NSSM_STATUS_CONFLICT:
+                what.append("a slot move named a slot twice, or one that another move reads")
             raise IndexError(f"nested_ssm: {'; '.join(what) or 'error'} (status {v})")
 
     def new_draft(self) -> torch.Tensor:

@@ -1,0 +1,415 @@
+"""The gated delta rule (nssm_delta_step, nssm_delta_scan) against its definition in fp64.
+
+Error bounds.  A rounding to a type of relative step eps is off by eps / 2 at most (fp32 2^-24,
+bf16 2^-8).
+
+* One decode token: every value is a dot product of N fp32 terms and a few more operations, so it
+  is off by at most (N + 16) 2^-24 of the sum of its terms' magnitudes (`_step_bounds`), plus the
+  rounding of the output.
+* A prompt: the state's own roundings are 2^-24 each, and no product is formed from operands
+  held to fewer than 17 bits, 2^-18 of each; a state remembers a handful of chunks, whose
+  errors add up, so the norm of the difference is below 8 2^-18 = 3.1e-5 of the state's at worst and
+  2^-18 sqrt(8) = 1.1e-5 for errors of random sign: 1e-5 is asked for.  An output may be formed
+  from operands rounded to bf16 (2^-8 at most, 2^-9 / sqrt(3) = 1.1e-3 in the mean square): its own
+  rounding (1.7e-3) and three such operands give 2.5e-3 of the norm; no value is off by more
+  than its own half step and 3 2^-8 of the root mean square of its row times 4.
+"""
+import pytest
+import torch
+
+import oracle.delta as OD
+
+pytestmark = pytest.mark.gpu
+STATE_TOL, Y_TOL = 1e-5, 2.5e-3
+
+
+def _unit(t):
+    return t / t.norm(dim=-1, keepdim=True)
+
+
+def _inputs(b, T, H, G, P, N, seed, dtype=torch.bfloat16, gdt=torch.float32, decay=0.3):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    return dict(q=_unit(r(b, T, G, N)).to(dtype), k=_unit(r(b, T, G, N)).to(dtype), v=r(b, T, H, P).to(dtype),
+                g=(-decay * torch.nn.functional.softplus(r(b, T, H))).to(gdt), beta=torch.sigmoid(r(b, T, H)).to(gdt),
+                s0=0.5 * r(b, H, P, N))
+
+
+def _rel(got, want):
+    n = float(want.double().norm())
+    return float((got.double() - want.double()).norm()) / n if n else float(got.double().norm())
+
+
+def _check_y(got, want, what=""):
+    assert torch.isfinite(got).all(), what
+    if not got.numel():
+        return
+    assert _rel(got, want) <= Y_TOL, f"{what}: {_rel(got, want):.2e}"
+    rms = want.square().mean(-1, keepdim=True).sqrt()
+    bound = 2.0 ** -8 * want.abs() + 12 * 2.0 ** -8 * rms + 1e-6
+    err = (got.double() - want).abs()
+    assert bool((err <= bound).all()), f"{what}: {float((err / bound).max()):.2f} of the bound"
+
+
+def _check_state(got, want, what=""):
+    assert torch.isfinite(got).all(), what
+    assert _rel(got, want) <= STATE_TOL, f"{what}: {_rel(got, want):.2e}"
+
+
+# ---------------------------------------------------------------- decode
+def _step_case(b, S, H, G, P, N, dtype, seed, gdt=torch.float32):
+    d = _inputs(b, 1, H, G, P, N, seed, dtype, gdt)
+    x = {n: d[n][:, 0] for n in ("q", "k", "v", "g", "beta")}
+    gen = torch.Generator(device="cuda").manual_seed(seed + 1)
+    state = torch.randn(S, H, P, N, generator=gen, device="cuda")
+    slots = torch.randperm(S, generator=gen, device="cuda")[:b].to(torch.int32)
+    return x, state, slots
+
+
+def _step_ref(x, state, slots, scale, out, rows):
+    """(state', out') in fp64 with the listed rows taken, and the bounds of both."""
+    S, y = state.double(), out.double()
+    N = state.shape[-1]
+    bS, by = torch.zeros_like(S), torch.zeros_like(y)
+    rep = state.shape[1] // x["q"].shape[1]
+    half = torch.finfo(out.dtype).eps / 2
+    for r in rows:
+        q, k = (x[n][r].double().repeat_interleave(rep, 0) for n in ("q", "k"))
+        v, g, beta = (x[n][r].double() for n in ("v", "g", "beta"))
+        old = torch.exp(g)[:, None, None] * S[slots[r]]
+        new, yr = OD.gated_delta_token(S[slots[r]], q, k, v, g, beta, scale)
+        e = (N + 16) * 2.0 ** -24
+        u = beta.abs()[:, None] * (v.abs() + (old.abs() * k.abs()[:, None]).sum(-1))     # >= |u|
+        bS[slots[r]] = e * (old.abs() + u[..., None] * k.abs()[:, None])
+        by[r] = half * yr.abs() + 2 * e * scale * ((old.abs() * q.abs()[:, None]).sum(-1) + u * (k.abs() * q.abs()).sum(-1)[:, None])
+        S[slots[r]], y[r] = new, yr
+    return S, y, bS, by
+
+
+def _check_step(state, out, ref):
+    S, y, bS, by = ref
+    assert bool(((state.double() - S).abs() <= bS).all())    # untouched slots: exactly
+    assert bool(((out.double() - y).abs() <= by).all())
+
+
+@pytest.mark.parametrize("b,S,H,G,P,N,dtype,gdt", [
+    (1, 1, 1, 1, 16, 64, torch.bfloat16, torch.float32),
+    (3, 7, 4, 2, 64, 128, torch.bfloat16, torch.bfloat16),
+    (5, 5, 6, 2, 80, 128, torch.float32, torch.float32),
+    (2, 9, 4, 4, 48, 64, torch.float32, torch.bfloat16),
+    (4, 6, 8, 1, 112, 128, torch.bfloat16, torch.float32),
+    (2, 3, 2, 1, 256, 128, torch.float32, torch.float32),
+    (70, 300, 2, 1, 128, 64, torch.bfloat16, torch.float32),
+])
+def test_step(b, S, H, G, P, N, dtype, gdt):
+    from nested_ssm_b200 import gated_delta_state_update
+    x, state, slots = _step_case(b, S, H, G, P, N, dtype, seed=b + P, gdt=gdt)
+    out = torch.full((b, H, P), 7.0, dtype=dtype, device="cuda")
+    ref = _step_ref(x, state, slots.long(), N ** -0.5, out, range(b))
+    got = gated_delta_state_update(state, x["q"], x["k"], x["v"], x["g"], x["beta"], state_batch_indices=slots, out=out)
+    assert got is out
+    _check_step(state, out, ref)
+
+
+def test_step_padded_out_of_range_and_repeated_rows():
+    from nested_ssm_b200 import gated_delta_state_update
+    x, state, slots = _step_case(8, 12, 4, 2, 64, 128, torch.bfloat16, seed=3)
+    slots[1] = -1           # padded
+    slots[4] = 12           # out of range
+    slots[6] = slots[2]     # named by an earlier row
+    slots[7] = -5
+    out = torch.full((8, 4, 64), 7.0, device="cuda", dtype=torch.bfloat16)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ref = _step_ref(x, state, slots.long(), 0.25, out, [0, 2, 3, 5])
+    gated_delta_state_update(state, x["q"], x["k"], x["v"], x["g"], x["beta"], 0.25, slots, out=out, status=status)
+    _check_step(state, out, ref)
+    assert int(status) == 1 | 8
+
+
+def test_step_pad_id_zero_and_index_column():
+    """vLLM's null block 0 as the pad id, and indices of shape [b, 1]."""
+    from nested_ssm_b200 import gated_delta_state_update
+    x, state, slots = _step_case(4, 9, 2, 2, 32, 64, torch.float32, seed=5)
+    slots = torch.tensor([3, 0, 8, 5], dtype=torch.int64, device="cuda")[:, None]
+    out = torch.zeros(4, 2, 32, device="cuda")
+    ref = _step_ref(x, state, slots[:, 0], 64 ** -0.5, out, [0, 2, 3])
+    gated_delta_state_update(state, x["q"], x["k"], x["v"], x["g"], x["beta"], None, slots, pad_slot_id=0, out=out)
+    _check_step(state, out, ref)
+
+
+def test_step_strided_and_unaligned_inputs():
+    """q, k, v, g, beta as slices of one projection (odd offsets), a state of spaced slots."""
+    from nested_ssm_b200 import gated_delta_state_update
+    b, S, H, G, P, N = 3, 5, 4, 2, 48, 128
+    x, state, slots = _step_case(b, S, H, G, P, N, torch.bfloat16, seed=8)
+    w = 2 * G * N + H * P + 2 * H + 3
+    proj = torch.zeros(b, w, dtype=torch.bfloat16, device="cuda")
+    at, v = 1, {}
+    for n in ("q", "k", "v", "g", "beta"):
+        size = x[n][0].numel()
+        proj[:, at:at + size] = x[n].reshape(b, -1).to(torch.bfloat16)
+        v[n] = proj[:, at:at + size].view(b, *x[n].shape[1:])
+        at += size
+    wide = torch.randn(S, 2, H, P, N, device="cuda")
+    wide[:, 1] = state
+    other = wide[:, 0].clone()
+    out = torch.zeros(b, 2 * H, P, device="cuda")[:, ::2]
+    ref = _step_ref(v, state, slots.long(), N ** -0.5, out, range(b))
+    gated_delta_state_update(wide[:, 1], v["q"], v["k"], v["v"], v["g"], v["beta"], None, slots, out=out)
+    _check_step(wide[:, 1], out, ref)
+    assert torch.equal(wide[:, 0], other)
+
+
+def test_step_empty_batch():
+    from nested_ssm_b200 import gated_delta_state_update
+    x, state, _ = _step_case(2, 2, 2, 1, 32, 64, torch.bfloat16, seed=9)
+    before = state.clone()
+    out = gated_delta_state_update(state, *(x[n][:0] for n in ("q", "k", "v", "g", "beta")))
+    assert out.shape == (0, 2, 32) and torch.equal(state, before)
+
+
+def test_step_state_offsets_beyond_32_bits():
+    from nested_ssm_b200 import gated_delta_state_update
+    H, P, N = 32, 128, 128
+    S = (1 << 31) // (H * P * N) + 3
+    state = torch.zeros(S, H, P, N, device="cuda")
+    x, small, _ = _step_case(2, 2, H, 16, P, N, torch.bfloat16, seed=10)
+    slots = torch.tensor([S - 1, 0], dtype=torch.int32, device="cuda")
+    state[S - 1], state[0] = small[0], small[1]
+    out = torch.zeros(2, H, P, device="cuda", dtype=torch.bfloat16)
+    ref = _step_ref(x, small, torch.arange(2), N ** -0.5, out, range(2))
+    gated_delta_state_update(state, x["q"], x["k"], x["v"], x["g"], x["beta"], None, slots, out=out)
+    _check_step(torch.stack([state[S - 1], state[0]]), out, ref)
+    assert float(state[1:S - 1].abs().max()) == 0.0
+
+
+# ---------------------------------------------------------------- prompts
+@pytest.mark.parametrize("b,T,H,G,P,N,init", [
+    (1, 1, 1, 1, 16, 64, False),
+    (2, 2, 2, 1, 32, 128, True),
+    (1, 15, 4, 2, 80, 128, True),
+    (3, 16, 2, 2, 64, 64, False),
+    (1, 17, 2, 1, 112, 64, True),
+    (2, 63, 4, 1, 48, 128, False),
+    (1, 64, 4, 2, 128, 128, True),
+    (1, 65, 2, 2, 96, 64, True),
+    (2, 127, 3, 3, 16, 128, True),
+    (1, 128, 2, 1, 256, 128, False),
+    (1, 129, 2, 1, 144, 64, True),
+    (2, 300, 4, 2, 80, 128, True),
+    (1, 1000, 2, 1, 64, 128, False),
+    (1, 777, 8, 8, 128, 64, True),
+])
+def test_scan(b, T, H, G, P, N, init):
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    d = _inputs(b, T, H, G, P, N, seed=T + P)
+    s0 = d["s0"] if init else None
+    y, S = gated_delta_chunk_scan(d["q"], d["k"], d["v"], d["g"], d["beta"], initial_states=s0, return_final_states=True)
+    yr, Sr = OD.gated_delta_scan(d["q"], d["k"], d["v"], d["g"], d["beta"], S0=s0)
+    _check_y(y, yr)
+    _check_state(S, Sr)
+
+
+@pytest.mark.parametrize("lens,H,G,P,N,init", [
+    ([5], 2, 1, 16, 64, True),
+    ([0, 1, 0, 64, 65, 0], 4, 2, 80, 128, True),
+    ([130, 1, 63, 200], 2, 2, 64, 128, False),
+    ([3] * 40, 2, 1, 48, 64, True),
+])
+def test_scan_packed(lens, H, G, P, N, init):
+    """Ragged sequences in one row, with empty ones, and rows behind the last that hold NaN: they are
+    neither read nor written."""
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    total = sum(lens) + 7
+    d = _inputs(1, total, H, G, P, N, seed=len(lens))
+    for n in ("q", "k", "v", "g", "beta"):
+        d[n][:, sum(lens):] = float("nan")
+    cu = torch.tensor([0] + lens, device="cuda").cumsum(0).to(torch.int32)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    s0 = torch.randn(len(lens), H, P, N, generator=g, device="cuda") if init else None
+    out = torch.full((1, total, H, P), 3.0, dtype=torch.bfloat16, device="cuda")
+    y, S = gated_delta_chunk_scan(d["q"], d["k"], d["v"], d["g"], d["beta"], initial_states=s0, cu_seqlens=cu,
+                                  return_final_states=True, out=out)
+    assert S.shape == (len(lens), H, P, N)
+    at = 0
+    for i, n in enumerate(lens):
+        x = [d[m][:, at:at + n] for m in ("q", "k", "v", "g", "beta")]
+        yr, Sr = OD.gated_delta_scan(*x, S0=None if s0 is None else s0[i:i + 1])
+        _check_y(y[:, at:at + n], yr, f"sequence {i}")
+        if n == 0:
+            assert torch.equal(S[i], s0[i] if init else torch.zeros_like(S[i]))
+        else:
+            _check_state(S[i], Sr[0], f"sequence {i}")
+        at += n
+    assert bool((y[:, at:] == 3.0).all())
+
+
+def test_scan_bad_bounds_are_skipped():
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    d = _inputs(1, 100, 2, 1, 32, 64, seed=4)
+    cu = torch.tensor([0, 70, 40, 100, 170], dtype=torch.int32, device="cuda")   # 1 descends, 3 leaves the rows
+    out = torch.full((1, 100, 2, 32), 3.0, dtype=torch.bfloat16, device="cuda")
+    fin = torch.full((4, 2, 32, 64), 5.0, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    # sequences 0 and 2 overlap: run each against a list in which the other is bad
+    gated_delta_chunk_scan(d["q"], d["k"], d["v"], d["g"], d["beta"], cu_seqlens=cu, out=out, final_states=fin,
+                           status=status)
+    assert int(status) == 8
+    assert bool((fin[1] == 5.0).all()) and bool((fin[3] == 5.0).all())
+    for s, (a, e) in ((0, (0, 70)), (2, (40, 100))):
+        _, Sr = OD.gated_delta_scan(*(d[m][:, a:e] for m in ("q", "k", "v", "g", "beta")))
+        _check_state(fin[s], Sr[0])
+
+
+@pytest.mark.parametrize("T", [0, 1, 70])
+def test_scan_states_in_place_and_without_tokens(T):
+    """final_states may be initial_states; without tokens the state stays."""
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    d = _inputs(2, T, 4, 2, 48, 128, seed=6)
+    s = d["s0"].clone()
+    y, S = gated_delta_chunk_scan(d["q"], d["k"], d["v"], d["g"], d["beta"], initial_states=s, return_final_states=True,
+                                  final_states=s)
+    assert S is s and y.shape == (2, T, 4, 48)
+    if T == 0:
+        assert torch.equal(s, d["s0"])
+        _, z = gated_delta_chunk_scan(d["q"], d["k"], d["v"], d["g"], d["beta"], return_final_states=True)
+        assert float(z.abs().max()) == 0.0
+    else:
+        _, Sr = OD.gated_delta_scan(d["q"], d["k"], d["v"], d["g"], d["beta"], S0=d["s0"])
+        _check_state(s, Sr)
+
+
+@pytest.mark.parametrize("gdt", [torch.float32, torch.bfloat16])
+def test_scan_strided_inputs_and_outputs(gdt):
+    """q / k / v as slices of one conv output, g / beta of one projection, y into a wider row."""
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    b, T, H, G, P, N = 2, 150, 4, 2, 80, 128
+    d = _inputs(b, T, H, G, P, N, seed=12, gdt=gdt)
+    conv = torch.cat([d[n].reshape(b, T, -1) for n in ("q", "k", "v")], -1)
+    q, k, v = conv.split([G * N, G * N, H * P], -1)
+    proj = torch.cat([d["g"], d["beta"]], -1)
+    wide = torch.zeros(b, T, 2 * H * P, dtype=torch.bfloat16, device="cuda")
+    out = wide[..., H * P:].view(b, T, H, P)
+    y, S = gated_delta_chunk_scan(q.view(b, T, G, N), k.view(b, T, G, N), v.view(b, T, H, P), proj[..., :H], proj[..., H:],
+                                  scale=0.3, initial_states=d["s0"], return_final_states=True, out=out)
+    assert y.data_ptr() == out.data_ptr() and float(wide[..., :H * P].abs().max()) == 0.0
+    yr, Sr = OD.gated_delta_scan(d["q"], d["k"], d["v"], d["g"], d["beta"], 0.3, d["s0"])
+    _check_y(y, yr)
+    _check_state(S, Sr)
+
+
+def test_scan_takes_unaligned_heads_and_broadcast_batches():
+    """Inputs the kernel cannot load as they lie (transposed heads, odd offsets, an expanded batch)
+    are laid out by the call."""
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    b, T, H, G, P, N = 2, 33, 4, 2, 16, 64
+    d = _inputs(b, T, H, G, P, N, seed=13)
+    q = d["q"].transpose(1, 2).contiguous().transpose(1, 2)
+    flat = torch.zeros(d["v"].numel() + 1, dtype=torch.bfloat16, device="cuda")
+    flat[1:] = d["v"].reshape(-1)
+    v = flat[1:].view(b, T, H, P)
+    k = d["k"][:1].expand(b, T, G, N)
+    beta = d["beta"][:, :, :1].expand(b, T, H)
+    y = gated_delta_chunk_scan(q, k, v, d["g"], beta)
+    yr, _ = OD.gated_delta_scan(q, k, v, d["g"], beta)
+    _check_y(y, yr)
+
+
+def test_scan_forgets_at_minus_infinity_and_keeps_small_decays_beside_large_ones():
+    """g = -inf forgets the state; a large decay early in a chunk does not blur the small ones behind
+    it."""
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    d = _inputs(1, 200, 2, 1, 32, 64, seed=14)
+    d["g"] = -0.01 * torch.rand(1, 200, 2, device="cuda")
+    d["g"][:, 3] = -3000.0
+    d["g"][:, 70, 0] = float("-inf")
+    d["g"][:, 128] = -50.0
+    d["s0"] *= 100
+    y, S = gated_delta_chunk_scan(d["q"], d["k"], d["v"], d["g"], d["beta"], initial_states=d["s0"], return_final_states=True)
+    yr, Sr = OD.gated_delta_scan(d["q"], d["k"], d["v"], d["g"], d["beta"], S0=d["s0"])
+    _check_y(y[:, 3:], yr[:, 3:])
+    _check_state(S, Sr)
+
+
+def test_scan_collinear_keys():
+    """The same key at every token with beta near 1: the system of a chunk is as far from the identity
+    as it gets, and u stays small only by cancellation."""
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    d = _inputs(1, 160, 2, 1, 32, 64, seed=15)
+    d["k"] = d["k"][:, :1].expand_as(d["k"]).contiguous()
+    d["beta"] = torch.full_like(d["beta"], 0.97)
+    d["g"] = torch.zeros_like(d["g"])
+    y, S = gated_delta_chunk_scan(d["q"], d["k"], d["v"], d["g"], d["beta"], initial_states=d["s0"], return_final_states=True)
+    yr, Sr = OD.gated_delta_scan(d["q"], d["k"], d["v"], d["g"], d["beta"], S0=d["s0"])
+    _check_y(y, yr)
+    _check_state(S, Sr)
+
+
+def test_scan_without_writes_keeps_the_state_exactly():
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    d = _inputs(1, 100, 2, 1, 48, 128, seed=16)
+    _, S = gated_delta_chunk_scan(d["q"], d["k"], d["v"], torch.zeros_like(d["g"]), torch.zeros_like(d["beta"]),
+                                  initial_states=d["s0"], return_final_states=True)
+    assert torch.equal(S, d["s0"])
+
+
+def test_scan_is_deterministic_and_sequences_are_independent():
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    d = _inputs(3, 190, 4, 2, 64, 128, seed=17)
+    x = [d[n] for n in ("q", "k", "v", "g", "beta")]
+    a = gated_delta_chunk_scan(*x, initial_states=d["s0"], return_final_states=True)
+    b = gated_delta_chunk_scan(*x, initial_states=d["s0"], return_final_states=True)
+    one = gated_delta_chunk_scan(*(t[1:2] for t in x), initial_states=d["s0"][1:2], return_final_states=True)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    assert torch.equal(a[0][1:2], one[0]) and torch.equal(a[1][1:2], one[1])
+
+
+def test_prefill_then_decode_equals_the_longer_prompt():
+    """A packed prefill whose states go to slots, then decode tokens on the slots."""
+    from nested_ssm_b200 import gated_delta_chunk_scan, gated_delta_state_update
+    b, T, extra, H, G, P, N = 3, 70, 4, 4, 2, 80, 128
+    d = _inputs(b, T + extra, H, G, P, N, seed=18)
+    x = [d[n] for n in ("q", "k", "v", "g", "beta")]
+    yr, Sr = OD.gated_delta_scan(*x)
+    pack = [t[:, :T].reshape(1, b * T, *t.shape[2:]) for t in x]
+    cu = torch.arange(0, b * T + 1, T, dtype=torch.int32, device="cuda")
+    _, S = gated_delta_chunk_scan(*pack, cu_seqlens=cu, return_final_states=True)
+    state = torch.zeros(8, H, P, N, device="cuda")
+    slots = torch.tensor([5, 0, 7], dtype=torch.int32, device="cuda")
+    state[slots.long()] = S
+    for t in range(T, T + extra):
+        y = gated_delta_state_update(state, *(z[:, t] for z in x), state_batch_indices=slots)
+        _check_y(y, yr[:, t])
+    _check_state(state[slots.long()], Sr)
+
+
+def test_on_another_stream_and_in_a_replayed_graph():
+    from nested_ssm_b200 import gated_delta_chunk_scan, gated_delta_state_update
+    d = _inputs(2, 90, 4, 2, 64, 128, seed=19)
+    names = ("q", "k", "v", "g", "beta")
+    x = [d[n] for n in names]
+    want = gated_delta_chunk_scan(*x, initial_states=d["s0"], return_final_states=True)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = gated_delta_chunk_scan(*x, initial_states=d["s0"], return_final_states=True)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    graphs, outs = [], []
+    for _ in range(2):      # two graphs, replayed in turn
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y, S = gated_delta_chunk_scan(*x, initial_states=d["s0"], return_final_states=True)
+            z = gated_delta_state_update(S, *(t[:, 0] for t in x))
+        graphs.append(g)
+        outs.append((y, S, z))
+    e = _inputs(2, 90, 4, 2, 64, 128, seed=20)
+    for n in names:
+        d[n].copy_(e[n])
+    d["s0"].copy_(e["s0"])
+    y, S = gated_delta_chunk_scan(*x, initial_states=d["s0"], return_final_states=True)
+    z = gated_delta_state_update(S, *(t[:, 0] for t in x))
+    for g in graphs + graphs:
+        g.replay()
+    for o in outs:
+        assert torch.equal(o[0], y) and torch.equal(o[1], S) and torch.equal(o[2], z)
