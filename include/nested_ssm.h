@@ -460,7 +460,7 @@ typedef struct {
   int32_t* status;        /* optional device word, bit 3 = bad cu_seqlens (that sequence is skipped) */
 } nssm_delta_scan_args;
 
-NSSM_API size_t nssm_delta_scan_workspace_bytes(int32_t batch, int32_t seqlen, int32_t nheads, int32_t headdim,
+NSSM_API size_t nssm_delta_scan_workspace_bytes(int32_t batch, int32_t seqlen, int32_t nheads, int32_t ngroups,
                                                 int32_t dstate, int32_t packed);
 NSSM_API int nssm_delta_scan(const nssm_delta_scan_args* args, void* stream);
 NSSM_API size_t nssm_sizeof_delta_scan_args(void);

@@ -2,7 +2,7 @@
 #include <cuda_runtime.h>
 #include <math.h>
 
-#include "nssm_delta.cuh"
+#include "nssm_delta_chunk.cuh"
 
 namespace nssm_host {
 int fail(int code, const char* fmt, ...);
@@ -33,6 +33,38 @@ int check_dims(int H, int G, int P, int N) {
 void slices(int P, int* ns, int* rows) {
   *ns = (P + 39) / 40;
   *rows = ((P + *ns - 1) / *ns + 3) / 4 * 4;
+}
+
+using nssm::kC;
+
+// Workspace chunks: of each sequence its own; a packed sequence of `len` tokens from token a on
+// takes ceil(len / C) from a / C + s on, which stay below seqlen / C + batch.
+int64_t ws_chunks(int batch, int seqlen, int packed) {
+  return packed ? (int64_t)seqlen / kC + batch : (int64_t)batch * ((seqlen + kC - 1) / kC);
+}
+
+template <int N>
+int launch_chunks(nssm::DeltaChunkParams& p, void* ws, cudaStream_t st) {
+  auto prep = nssm::delta_prep_kernel<N>;
+  auto walk = p.s.G * p.tile_groups * p.s.B > 296 ? nssm::delta_chunk_kernel<N, 3> : nssm::delta_chunk_kernel<N, 2>;
+  p.img = static_cast<unsigned char*>(ws);
+  p.blk = p.img + (int64_t)p.chunks * p.s.G * nssm::kImgBytes<N>;
+  const int smem = nssm::ChunkSmem<N>::bytes(p.heads);
+  cudaError_t e = cudaFuncSetAttribute(prep, cudaFuncAttributeMaxDynamicSharedMemorySize, nssm::PrepSmem<N>::kBytes);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(walk, cudaFuncAttributeMaxDynamicSharedMemorySize, nssm::ChunkSmem<N>::bytes(nssm::kWarps));
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(walk, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(NSSM_ERR_CUDA, "delta scan: %s", cudaGetErrorString(e));
+  }
+  if (p.chunks > 0) {
+    prep<<<dim3(p.chunks, p.s.G), nssm::kPrepThreads, nssm::PrepSmem<N>::kBytes, st>>>(p);
+    const int rc = launched("delta_prep_kernel");
+    if (rc) return rc;
+  }
+  walk<<<dim3(p.s.G * p.tile_groups, p.s.B), nssm::kWarps * 32, smem, st>>>(p);
+  return launched("delta_chunk_kernel");
 }
 
 }  // namespace
@@ -85,7 +117,12 @@ int nssm_delta_step(const nssm_delta_step_args* a, void* stream) {
   return launched("delta_step_kernel");
 }
 
-size_t nssm_delta_scan_workspace_bytes(int32_t, int32_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
+size_t nssm_delta_scan_workspace_bytes(int32_t batch, int32_t seqlen, int32_t nheads, int32_t ngroups, int32_t dstate,
+                                       int32_t packed) {
+  if (batch <= 0 || seqlen <= 0 || nheads <= 0 || ngroups <= 0) return 0;
+  const size_t img = dstate == 64 ? nssm::kImgBytes<64> : nssm::kImgBytes<128>;
+  return (size_t)ws_chunks(batch, seqlen, packed) * (ngroups * img + (size_t)nheads * nssm::kBlkBytes);
+}
 
 int nssm_delta_scan(const nssm_delta_scan_args* a, void* stream) {
   if (!a) return fail(NSSM_ERR_INVALID, "args is NULL");
@@ -110,7 +147,6 @@ int nssm_delta_scan(const nssm_delta_scan_args* a, void* stream) {
     return fail(NSSM_ERR_INVALID, "final_stride_b smaller than a state");
   nssm::DeltaScanParams p{};
   p.B = a->batch; p.T = a->seqlen; p.H = a->nheads; p.G = a->ngroups; p.P = a->headdim;
-  slices(p.P, &p.ns, &p.rows);
   p.g_bf16 = a->g_dtype == NSSM_BF16; p.beta_bf16 = a->beta_dtype == NSSM_BF16;
   p.scale = a->scale;
   p.q = static_cast<const __nv_bfloat16*>(a->q); p.q_b = a->q_stride_b; p.q_t = a->q_stride_t;
@@ -123,13 +159,21 @@ int nssm_delta_scan(const nssm_delta_scan_args* a, void* stream) {
   p.y = static_cast<__nv_bfloat16*>(a->y); p.y_b = a->y_stride_b; p.y_t = a->y_stride_t;
   p.fin = a->final_states; p.fin_b = a->final_stride_b;
   p.status = a->status;
-  const dim3 grid(p.H * p.ns, p.B);
+  p.polls = nssm::kSpinLimit;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->dstate == 64)
-    nssm::delta_scan_kernel<64><<<grid, p.rows * 8, 0, st>>>(p);
-  else
-    nssm::delta_scan_kernel<128><<<grid, p.rows * 8, 0, st>>>(p);
-  return launched("delta_scan_kernel");
+  const size_t need = nssm_delta_scan_workspace_bytes(a->batch, a->seqlen, a->nheads, a->ngroups, a->dstate,
+                                                    a->cu_seqlens != nullptr);
+  if (need && (!a->workspace || !al(a->workspace, 16) || a->workspace_bytes < need))
+    return fail(NSSM_ERR_INVALID, "a 16-byte aligned workspace of %zu bytes is needed (got %zu)", need, a->workspace_bytes);
+  nssm::DeltaChunkParams c{};
+  c.s = p;
+  c.chunks = (int)ws_chunks(a->batch, a->seqlen, a->cu_seqlens != nullptr);
+  c.per_seq = (a->seqlen + kC - 1) / kC;
+  c.tiles = a->headdim / 16;
+  c.tile_groups = (a->nheads / a->ngroups * c.tiles + nssm::kWarps - 1) / nssm::kWarps;
+  // four tiles from a multiple of four on lie in one or two heads of two tiles or more
+  c.heads = c.tiles == 1 ? nssm::kWarps : c.tiles % nssm::kWarps ? 2 : 1;
+  return a->dstate == 64 ? launch_chunks<64>(c, a->workspace, st) : launch_chunks<128>(c, a->workspace, st);
 }
 
 }  // extern "C"

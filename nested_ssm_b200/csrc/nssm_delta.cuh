@@ -1,6 +1,6 @@
 // The gated delta rule on states S[headdim][dstate] (fp32), per value head h:
 //   S <- e^g S;  u = beta (v - S k);  S <- S + u k^T;  y = scale S q
-// Decode (delta_step_kernel) and prompts token by token (delta_scan_kernel).
+// One decode token (delta_step_kernel); nssm_delta_chunk.cuh takes prompts.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(320) delta_step_kernel(const DeltaStepParams p
 }
 
 struct DeltaScanParams {
-  int B, T, H, G, P, ns, rows;
+  int B, T, H, G, P;
   int g_bf16, beta_bf16;
   float scale;
   const __nv_bfloat16 *q, *k, *v;
@@ -134,6 +134,7 @@ struct DeltaScanParams {
   float* fin;
   int64_t fin_b;
   int32_t* status;
+  uint32_t polls;        // limit of a bounded wait
 };
 
 // Tokens [t0, t0 + len) of sequence s (in its own batch row, or packed); false: bad bounds.
@@ -145,90 +146,6 @@ __device__ __forceinline__ bool delta_seq(const DeltaScanParams& p, int s, int* 
   const int a = p.cu[s], e = p.cu[s + 1];
   *batch = 0; *t0 = a; *len = e - a;
   return a >= 0 && e >= a && e <= p.T;
-}
-
-constexpr int kScanTok = 16;   // tokens staged at a time
-
-// A prompt token by token, the state in registers (the layout of delta_step_kernel); q and k of
-// kScanTok tokens are staged as fp32 in shared memory.
-template <int N>
-__global__ void __launch_bounds__(320) delta_scan_kernel(const DeltaScanParams p) {
-  constexpr int V = N / 32;
-  __shared__ float sq[kScanTok][N], sk[kScanTok][N];
-  __shared__ float sv[kScanTok][40], sg[kScanTok], sb[kScanTok], skq[kScanTok];
-  const int s = blockIdx.y, h = blockIdx.x / p.ns, slice = blockIdx.x - h * p.ns;
-  const int tid = threadIdx.x, l8 = tid & 7, rl = tid >> 3;
-  const int r = slice * p.rows + rl;
-  const bool live = r < p.P;
-  int batch, t0, len;
-  if (!delta_seq(p, s, &batch, &t0, &len)) {
-    if (p.status && blockIdx.x == 0 && tid == 0) atomicOr(p.status, STATUS_CONFLICT);
-    return;
-  }
-  const int64_t off = ((int64_t)h * p.P + (live ? r : 0)) * N;
-  float4 st[V];
-#pragma unroll
-  for (int c = 0; c < V; ++c)
-    st[c] = p.init ? reinterpret_cast<const float4*>(p.init + s * p.init_b + off)[l8 + 8 * c]
-                   : make_float4(0.f, 0.f, 0.f, 0.f);
-  const int kh = h / (p.H / p.G);
-  for (int tb = 0; tb < len; tb += kScanTok) {
-    const int nt = min(kScanTok, len - tb);
-    __syncthreads();
-    for (int i = tid; i < nt * (N / 2); i += blockDim.x) {
-      const int t = i / (N / 2), n = 2 * (i - t * (N / 2));
-      const int64_t tok = t0 + tb + t;
-      const float2 fk = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p.k + batch * p.k_b + tok * p.k_t + kh * N + n));
-      const float2 fq = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p.q + batch * p.q_b + tok * p.q_t + kh * N + n));
-      sk[t][n] = fk.x; sk[t][n + 1] = fk.y;
-      sq[t][n] = fq.x; sq[t][n + 1] = fq.y;
-    }
-    for (int i = tid; i < nt * p.rows; i += blockDim.x) {
-      const int t = i / p.rows, c = i - t * p.rows;
-      const int64_t tok = t0 + tb + t;
-      sv[t][c] = slice * p.rows + c < p.P ? __bfloat162float(p.v[batch * p.v_b + tok * p.v_t + h * p.P + slice * p.rows + c]) : 0.0f;
-    }
-    if (tid < nt) {
-      const int64_t tok = t0 + tb + tid;
-      sg[tid] = expf(dl_ld(p.g, batch * p.g_b + tok * p.g_t + h, p.g_bf16));
-      sb[tid] = dl_ld(p.beta, batch * p.beta_b + tok * p.beta_t + h, p.beta_bf16);
-    }
-    __syncthreads();
-    for (int t = tid >> 5; t < nt; t += blockDim.x >> 5) {   // k.q of each token, one warp each
-      float a = 0.0f;
-      for (int n = tid & 31; n < N; n += 32) a = fmaf(sk[t][n], sq[t][n], a);
-#pragma unroll
-      for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-      if ((tid & 31) == 0) skq[t] = a;
-    }
-    __syncthreads();
-    for (int t = 0; t < nt; ++t) {
-      float a = 0.0f, c2 = 0.0f;
-      const float eg = sg[t];
-      float4 kk[V];
-#pragma unroll
-      for (int c = 0; c < V; ++c) {
-        kk[c] = reinterpret_cast<const float4*>(sk[t])[l8 + 8 * c];
-        const float4 qq = reinterpret_cast<const float4*>(sq[t])[l8 + 8 * c];
-        st[c].x *= eg; st[c].y *= eg; st[c].z *= eg; st[c].w *= eg;
-        a = dot4(st[c], kk[c], a);
-        c2 = dot4(st[c], qq, c2);
-      }
-      a = sum8(a); c2 = sum8(c2);
-      const float u = sb[t] * (sv[t][rl] - a);
-#pragma unroll
-      for (int c = 0; c < V; ++c) {
-        st[c].x = fmaf(u, kk[c].x, st[c].x); st[c].y = fmaf(u, kk[c].y, st[c].y);
-        st[c].z = fmaf(u, kk[c].z, st[c].z); st[c].w = fmaf(u, kk[c].w, st[c].w);
-      }
-      if (l8 == 0 && live)
-        p.y[batch * p.y_b + (int64_t)(t0 + tb + t) * p.y_t + h * p.P + r] =
-            __float2bfloat16_rn(p.scale * fmaf(u, skq[t], c2));
-    }
-  }
-  if (p.fin && live)
-#pragma unroll
-    for (int c = 0; c < V; ++c) reinterpret_cast<float4*>(p.fin + s * p.fin_b + off)[l8 + 8 * c] = st[c];
 }
 
 }  // namespace nssm

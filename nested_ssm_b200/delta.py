@@ -162,7 +162,7 @@ def gated_delta_chunk_scan(q, k, v, g, beta, scale: float | None = None, initial
     _check_status(status)
     dev = _require_cuda(q, k, v, g, beta, cu_seqlens, initial_states, out, final_states, status)
     lib = _lib.load()
-    nbytes = lib.nssm_delta_scan_workspace_bytes(n, T, H, P, N, int(cu_seqlens is not None))
+    nbytes = lib.nssm_delta_scan_workspace_bytes(n, T, H, G, N, int(cu_seqlens is not None))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     a = _lib.NssmDeltaScanArgs(
         n, T, H, G, P, N, nssm_dtype(g.dtype), nssm_dtype(beta.dtype), N ** -0.5 if scale is None else float(scale), 0,
