@@ -470,7 +470,8 @@ NSSM_API size_t nssm_sizeof_delta_scan_args(void);
  * each); a move takes them all.  The list of moves is checked on the device before anything is
  * written: a slot out of range (bit 0 of *status), a destination named twice or a destination
  * that another move reads (bit 3) drops those moves and no others, so the result does not depend
- * on the order of execution.  A move of a slot onto itself does nothing. */
+ * on the order of execution.  A move of a slot onto itself does nothing.  The lists and new_slots are
+ * arrays of their own, apart from each other and from the buffers. */
 typedef struct {
   void* base;             /* element (o, s, 0) at base + o*outer_stride + s*slot_stride, bytes */
   int64_t outer_stride;

@@ -8,7 +8,10 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import threading
+
+import torch
 
 from . import build as _build
 
@@ -165,6 +168,46 @@ class NssmBeamArgs(C.Structure):
     ]
 
 
+def packer(struct_type):
+    """``pack(*fields)`` -> the bytes of a ``struct_type`` (0 for a NULL pointer): the small calls
+    are bound by the host, and this costs a fifth of filling a ctypes structure."""
+    code = {C.c_int32: "i", C.c_int64: "q", C.c_float: "f", C.c_void_p: "P", C.c_size_t: "N"}
+    s = struct.Struct("@" + "".join(code[t] for _, t in struct_type._fields_))
+    if s.size != C.sizeof(struct_type):
+        raise RuntimeError(f"layout of {struct_type.__name__}")
+    return s.pack
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def stream_of(index: int) -> int:
+    """cudaStream_t of device ``index``'s current stream."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def device_index(*tensors) -> int:
+    """The one CUDA device of the tensors (None among them is skipped)."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise RuntimeError(f"tensors on different devices: {tensors[0].device} vs {t.device}")
+    if dev < 0 or not tensors[0].is_cuda:
+        raise RuntimeError("nested_ssm_b200 ops take CUDA tensors only (no CPU fallback)")
+    return dev
+
+
+def call(fn, dev: int, *args) -> None:
+    """``fn(*args, stream)`` on device ``dev`` and its current stream."""
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, stream_of(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream_of(dev))
+    if rc:
+        check(rc)
+
+
 MAX_SLOT_BUFFERS, MAX_SLOT_ROWS, MAX_MOVE_SLOTS = 24, 4096, 131072
 MAX_BEAMS, MAX_BEAM_OUT = 64, 128
 
@@ -180,6 +223,8 @@ def lib_path() -> str:
 def load(auto_build: bool = True) -> C.CDLL:
     """Load (building first if stale and nvcc is present) the C-ABI library."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -222,10 +267,10 @@ def load(auto_build: bool = True) -> C.CDLL:
             "nssm_verify_step": (C.c_int, [P_pool, P_args, C.POINTER(NssmTokenArgs), vp]),
             "nssm_commit_step": (C.c_int, [P_pool, P_args, C.POINTER(NssmTokenArgs), vp]),
             "nssm_sizeof_token_args": (sz, []),
-            "nssm_delta_step": (C.c_int, [C.POINTER(NssmDeltaStepArgs), vp]),
+            "nssm_delta_step": (C.c_int, [vp, vp]),
             "nssm_sizeof_delta_step_args": (sz, []),
             "nssm_delta_scan_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
-            "nssm_delta_scan": (C.c_int, [C.POINTER(NssmDeltaScanArgs), vp]),
+            "nssm_delta_scan": (C.c_int, [vp, vp]),
             "nssm_sizeof_delta_scan_args": (sz, []),
             "nssm_sizeof_slot_buffer": (sz, []),
             "nssm_slot_workspace_bytes": (sz, [i32]),
@@ -233,7 +278,7 @@ def load(auto_build: bool = True) -> C.CDLL:
             "nssm_slot_reorder": (C.c_int, [vp, i32, i32, vp, vp, i32, i32, i32, vp, vp, sz, vp, vp]),
             "nssm_slot_compact": (C.c_int, [vp, i32, i32, vp, i32, i32, vp, vp, sz, vp, vp]),
             "nssm_beam_workspace_bytes": (sz, [i32, i32, i32, i32, i32]),
-            "nssm_beam_select": (C.c_int, [C.POINTER(NssmBeamArgs), vp]),
+            "nssm_beam_select": (C.c_int, [vp, vp]),
             "nssm_sizeof_beam_args": (sz, []),
         }
         for name, (res, args) in sig.items():

@@ -2,14 +2,13 @@
 :func:`~nested_ssm_b200.slots.reorder_slots`."""
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
 from . import _lib
 from .delta import _no_grad
-from .ops import _ptr, _require_cuda, _stream
 from .pool import nssm_dtype
+
+_pack = _lib.packer(_lib.NssmBeamArgs)
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_out: int | None = None, finished=None,
@@ -45,18 +44,19 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_out: int | None 
         scores = scores.contiguous()
     if finished is not None and not finished.is_contiguous():
         finished = finished.contiguous()
-    dev = _require_cuda(logits, scores, finished)
+    dev = _lib.device_index(logits, scores, finished)
     lib = _lib.load()
-    out_s = torch.empty(b, n, dtype=torch.float32, device=dev)
-    out_p = torch.empty(b, n, dtype=torch.int32, device=dev)
-    out_t = torch.empty(b, n, dtype=torch.int32, device=dev)
-    out_f = torch.empty(b, n, dtype=torch.bool, device=dev) if eos_token_id is not None else None
+    where = logits.device
+    out_s = torch.empty(b, n, dtype=torch.float32, device=where)
+    out_p = torch.empty(b, n, dtype=torch.int32, device=where)
+    out_t = torch.empty(b, n, dtype=torch.int32, device=where)
+    out_f = torch.empty(b, n, dtype=torch.bool, device=where) if eos_token_id is not None else None
     dt = nssm_dtype(logits.dtype)
     nbytes = lib.nssm_beam_workspace_bytes(b, K, V, n, dt)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    a = _lib.NssmBeamArgs(b, K, V, n, dt, -1 if eos_token_id is None else int(eos_token_id), logits.data_ptr(),
-                          logits.stride(0), logits.stride(1), scores.data_ptr(), _ptr(finished), out_s.data_ptr(),
-                          out_p.data_ptr(), out_t.data_ptr(), _ptr(out_f), ws.data_ptr(), nbytes)
-    with torch.cuda.device(dev):
-        _lib.check(lib.nssm_beam_select(C.byref(a), _stream(dev)))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=where)
+    l0, l1, _ = logits.stride()
+    a = _pack(b, K, V, n, dt, -1 if eos_token_id is None else int(eos_token_id), logits.data_ptr(), l0, l1,
+              scores.data_ptr(), 0 if finished is None else finished.data_ptr(), out_s.data_ptr(), out_p.data_ptr(),
+              out_t.data_ptr(), 0 if out_f is None else out_f.data_ptr(), ws.data_ptr(), nbytes)
+    _lib.call(lib.nssm_beam_select, dev, a)
     return (out_s, out_p, out_t) if out_f is None else (out_s, out_p, out_t, out_f)

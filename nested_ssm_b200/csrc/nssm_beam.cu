@@ -13,13 +13,15 @@ int fail(int code, const char* fmt, ...);
 
 namespace nssm {
 
-constexpr int kBeamThreads = 256;
-constexpr int kVecs = 4;                 // 16-byte pieces of a segment per thread
+constexpr int kBeamThreads = 256, kBeamWarps = kBeamThreads / 32;
+constexpr int kVecs = 4;                 // 16-byte pieces per thread and step
 constexpr int kMaxOut = NSSM_MAX_BEAM_OUT;
 constexpr float kNegInf = -INFINITY;
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct BeamParams {
-  int b, K, V, n, splits, bf16, eos;
+  int b, K, V, n, eos;
+  int splits, steps;   // CTAs of a row, steps of kBeamThreads * kVecs pieces each
   const void* logits;
   int64_t l_b, l_k;
   const float* scores;
@@ -45,130 +47,210 @@ __device__ __forceinline__ float unorder32(uint32_t o) {
 __device__ __forceinline__ uint64_t key_of(float x, int token) {
   return ((uint64_t)order32(x) << 32) | (uint32_t)~token;
 }
-__device__ __forceinline__ float masked(float x) { return isfinite(x) ? x : kNegInf; }
+__device__ __forceinline__ float ex2(float x) {   // 2^x, 2 ulp
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
-// The nth (1-based) largest of kBeamThreads distinct values, by counting for each how many are
-// larger; n <= kBeamThreads.  K: a type with operator<.
-template <typename Key>
-__device__ __forceinline__ Key nth_of_block(Key mine, int n, Key* sh, Key* result) {
+// The nth (1-based) largest of the CTA's values (n <= kBeamThreads), by counting for each how many
+// are larger or equal and earlier.
+__device__ __forceinline__ uint64_t nth_of_block(uint64_t mine, int n, uint64_t* sh, uint64_t* result) {
   sh[threadIdx.x] = mine;
   __syncthreads();
   int rank = 0;
-  for (int i = 0; i < kBeamThreads; ++i) rank += mine < sh[i];
+#pragma unroll 8
+  for (int i = 0; i < kBeamThreads; i += 2) {
+    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(sh + i);
+    rank += (v.x > mine) + (v.y > mine);
+    rank += (v.x == mine && i < (int)threadIdx.x) + (v.y == mine && i + 1 < (int)threadIdx.x);
+  }
   if (rank == n - 1) *result = mine;
   __syncthreads();
   return *result;
 }
 
-// Segment of a row: a thread keeps kVecs 16-byte pieces in registers, so the max, the sum and
-// the candidates all come from one read.  A lower bound of the nout-th best candidate is the
-// nout-th largest of the threads' own maxima; only the few candidates above it are ranked.
+// A part of a row, a step of kBeamThreads * kVecs 16-byte pieces at a time; the max, the sum and
+// the candidates of a step all come from one read into registers.  Only values that reach a lower
+// bound of the nout-th best so far become candidates: at first the nout-th best of a few maxima of
+// each warp, then the nout-th best itself.  Any bound is safe; one that lets through too many
+// (sorted or constant logits) is replaced by the nout-th largest of the threads' own best keys,
+// which lets through at most nout threads' values.
 template <bool BF16>
-__global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const BeamParams p) {
+__global__ void __launch_bounds__(kBeamThreads, 4) beam_scan_kernel(const BeamParams p) {
   constexpr int E = BF16 ? 8 : 4;                       // elements of a 16-byte piece
-  constexpr int kSeg = kBeamThreads * kVecs * E;
+  constexpr int kStep = kBeamThreads * kVecs * E;
   constexpr int kCap = kMaxOut * kVecs * E;             // candidates of kMaxOut threads
-  __shared__ uint64_t sh[kBeamThreads];
-  __shared__ uint64_t list[kCap];
-  __shared__ float red[kBeamThreads / 32];
+  __shared__ __align__(16) uint64_t sh[kBeamThreads];
+  __shared__ uint64_t list[kCap + kMaxOut], cur[kMaxOut];
+  __shared__ float red[kBeamWarps], rsum[kBeamWarps];
   __shared__ uint64_t nth;
   __shared__ int count;
   const int row = blockIdx.y, bi = row / p.K, ki = row - bi * p.K, split = blockIdx.x;
   if (p.fin && p.fin[row]) return;                      // the merge knows its one candidate
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int es = BF16 ? 2 : 4;
+  constexpr int es = BF16 ? 2 : 4;
   const char* base = static_cast<const char*>(p.logits) + (bi * p.l_b + ki * p.l_k) * es;
   // pieces are 16-byte aligned in memory: piece 0 of the row may begin before the row does
   const int lead = (int)((reinterpret_cast<uintptr_t>(base) & 15) / es);
-  float x[kVecs * E];
-  int tok0[kVecs];
-  float mx = kNegInf;
+  const int steps = min(p.steps, (p.V + lead + kStep - 1) / kStep - split * p.steps);
+  float m = kNegInf, sum = 0.0f;                        // this thread's running maximum and sum
+  int have = 0;                                         // entries of cur, sorted
+  if (tid == 0) count = 0;
+  for (int st = 0; st < steps; ++st) {
+    const int first = (split * p.steps + st) * kStep + tid * E - lead;
+    float x[kVecs * E];
+    float mx = kNegInf;
+    bool odd = false;
 #pragma unroll
-  for (int c = 0; c < kVecs; ++c) {
-    const int t0 = split * kSeg + (c * kBeamThreads + tid) * E - lead;
-    tok0[c] = t0;
-    if (t0 >= 0 && t0 + E <= p.V) {
-      const uint4 r = __ldg(reinterpret_cast<const uint4*>(base + (int64_t)t0 * es));
-      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    for (int c = 0; c < kVecs; ++c) {
+      const int t0 = first + c * kBeamThreads * E;
+      if (t0 >= 0 && t0 + E <= p.V) {
+        const uint4 r = __ldg(reinterpret_cast<const uint4*>(base + (int64_t)t0 * es));
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (BF16) {
-          x[c * E + 2 * i] = __uint_as_float(w[i] << 16);
-          x[c * E + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        } else {
-          x[c * E + i] = __uint_as_float(w[i]);
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (BF16) {
+            x[c * E + 2 * i] = __uint_as_float(w[i] << 16);
+            x[c * E + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+          } else {
+            x[c * E + i] = __uint_as_float(w[i]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const int t = t0 + i;
+          x[c * E + i] = kNegInf;
+          if (t >= 0 && t < p.V)
+            x[c * E + i] = BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[t])
+                                : reinterpret_cast<const float*>(base)[t];
         }
       }
-    } else {
+    }
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int t = t0 + i;
-        x[c * E + i] = kNegInf;
-        if (t >= 0 && t < p.V)
-          x[c * E + i] = BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[t])
-                              : reinterpret_cast<const float*>(base)[t];
+    for (int i = 0; i < kVecs * E; ++i) {
+      odd |= !(x[i] <= 3.402823466e38f);
+      mx = fmaxf(mx, x[i]);
+    }
+    if (odd) {       // NaN and +inf count as masked
+      mx = kNegInf;
+#pragma unroll
+      for (int i = 0; i < kVecs * E; ++i) {
+        if (!(x[i] <= 3.402823466e38f)) x[i] = kNegInf;
+        mx = fmaxf(mx, x[i]);
       }
     }
+    if (mx > m) {
+      sum *= ex2((m - mx) * kLog2e);
+      m = mx;
+    }
+    if (m != kNegInf) {
+      // the difference first: x and m may both be the type's lowest value
+      float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      x[c * E + i] = masked(x[c * E + i]);
-      mx = fmaxf(mx, x[c * E + i]);
+      for (int i = 0; i < kVecs * E; ++i) s4[i & 3] += ex2((x[i] - m) * kLog2e);
+      sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+    }
+    // the bound
+    float tau;
+    if (have == p.n) {
+      tau = unorder32((uint32_t)(cur[p.n - 1] >> 32));
+    } else {
+      const int t = min(32, (2 * p.n + kBeamWarps - 1) / kBeamWarps);   // maxima of each warp
+      uint32_t mine = order32(mx);
+      for (int k = 0; k < t; ++k) {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, mine);
+        if (lane == 0) sh[warp * t + k] = top;
+        const int who = __ffs(__ballot_sync(0xffffffffu, mine == top)) - 1;
+        if (lane == who) mine = 0;
+      }
+      __syncthreads();
+      int rank = 0;
+      const uint64_t v = tid < kBeamWarps * t ? sh[tid] : 0;
+      for (int i = 0; i < kBeamWarps * t; ++i) rank += sh[i] > v || (sh[i] == v && i < tid);
+      if (tid < kBeamWarps * t && rank == p.n - 1) nth = v;
+      __syncthreads();
+      tau = unorder32((uint32_t)nth);
+      if (!(tau >= kNegInf)) tau = kNegInf;
+    }
+    int mycount = 0;
+    if (mx >= tau)
+#pragma unroll
+      for (int i = 0; i < kVecs * E; ++i) {
+        const int tk = first + (i / E) * kBeamThreads * E + i % E;
+        if (x[i] >= tau && tk >= 0 && tk < p.V) ++mycount;
+      }
+    int at = mycount ? atomicAdd(&count, mycount) : 0;
+    __syncthreads();
+    int found = count;
+    uint64_t least = 0;
+    const bool many = found > max(256, 4 * p.n);
+    if (many) {
+      uint64_t best = 0;
+#pragma unroll
+      for (int i = 0; i < kVecs * E; ++i) {
+        const int tk = first + (i / E) * kBeamThreads * E + i % E;
+        const uint64_t k = tk >= 0 && tk < p.V ? key_of(x[i], tk) : 0;
+        best = k > best ? k : best;
+      }
+      least = nth_of_block(best, p.n, sh, &nth);
+      mycount = 0;
+      if (best >= least)
+#pragma unroll
+        for (int i = 0; i < kVecs * E; ++i) {
+          const int tk = first + (i / E) * kBeamThreads * E + i % E;
+          if (tk >= 0 && tk < p.V && key_of(x[i], tk) >= least) ++mycount;
+        }
+      if (tid == 0) count = 0;
+      __syncthreads();
+      at = mycount ? atomicAdd(&count, mycount) : 0;
+      __syncthreads();
+      found = count;
+    }
+    if (mycount)
+#pragma unroll
+      for (int i = 0; i < kVecs * E; ++i) {
+        const int tk = first + (i / E) * kBeamThreads * E + i % E;
+        if (tk < 0 || tk >= p.V) continue;
+        if (many ? key_of(x[i], tk) >= least : x[i] >= tau) list[at++] = key_of(x[i], tk);
+      }
+    __syncthreads();     // every thread has read count
+    if (found) {
+      for (int i = tid; i < have; i += kBeamThreads) list[found + i] = cur[i];
+      if (tid == 0) count = 0;
+      __syncthreads();
+      const int total = found + have;
+      for (int i = tid; i < total; i += kBeamThreads) {
+        const uint64_t k = list[i];
+        int rank = 0;
+        for (int j = 0; j < total; ++j) rank += list[j] > k;
+        if (rank < p.n) cur[rank] = k;
+      }
+      have = min(total, p.n);
+      __syncthreads();
     }
   }
-  // the thread's best key (0: no token of the row)
-  uint64_t best = 0;
+  uint64_t* out = p.cand + ((int64_t)row * p.splits + split) * p.n;
+  for (int i = tid; i < p.n; i += kBeamThreads) out[i] = i < have ? cur[i] : 0;
+  // the part's maximum and sum
+  float mm = m;
 #pragma unroll
-  for (int c = 0; c < kVecs; ++c)
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int t = tok0[c] + i;
-      const uint64_t k = (t >= 0 && t < p.V) ? key_of(x[c * E + i], t) : 0;
-      best = k > best ? k : best;
-    }
-  float m = mx;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane == 0) red[warp] = m;
-  if (tid == 0) count = 0;
+  for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+  if (lane == 0) red[warp] = mm;
   __syncthreads();
-  m = red[0];
+  mm = red[0];
 #pragma unroll
-  for (int w = 1; w < kBeamThreads / 32; ++w) m = fmaxf(m, red[w]);
-  __syncthreads();
-  float sum = 0.0f;
-  if (m != kNegInf)
-#pragma unroll
-    for (int i = 0; i < kVecs * E; ++i) sum += expf(x[i] - m);
+  for (int w = 1; w < kBeamWarps; ++w) mm = fmaxf(mm, red[w]);
+  if (mm != kNegInf) sum *= ex2((m - mm) * kLog2e);     // 0 for a thread without a value
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) red[warp] = sum;
-  // threads without a token get distinct keys below every real one (those have bit 63..32 >= 0x007fffff)
-  const uint64_t tau = nth_of_block<uint64_t>(best ? best : (uint64_t)tid, p.n, sh, &nth);
+  if (lane == 0) rsum[warp] = sum;
+  __syncthreads();
   if (tid == 0) {
     float s = 0.0f;
-    for (int w = 0; w < kBeamThreads / 32; ++w) s += red[w];
-    p.part[(int64_t)row * p.splits + split] = make_float2(m, s);
-  }
-  if (best && best >= tau)
-#pragma unroll
-    for (int c = 0; c < kVecs; ++c)
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int t = tok0[c] + i;
-        if (t < 0 || t >= p.V) continue;
-        const uint64_t k = key_of(x[c * E + i], t);
-        if (k >= tau) list[atomicAdd(&count, 1)] = k;
-      }
-  __syncthreads();
-  const int cnt = count;
-  uint64_t* out = p.cand + ((int64_t)row * p.splits + split) * p.n;
-  for (int i = tid; i < p.n; i += kBeamThreads)
-    if (i >= cnt) out[i] = 0;
-  for (int i = tid; i < cnt; i += kBeamThreads) {
-    const uint64_t k = list[i];
-    int rank = 0;
-    for (int j = 0; j < cnt; ++j) rank += list[j] > k;
-    if (rank < p.n) out[rank] = k;
+    for (int w = 0; w < kBeamWarps; ++w) s += rsum[w];
+    p.part[(int64_t)row * p.splits + split] = make_float2(mm, s);
   }
 }
 
@@ -195,9 +277,9 @@ static_assert(NSSM_MAX_BEAMS <= 1 << kBeamBits && kBeamBits + kTokenBits == 32, 
 // has anything above the nout-th best so far at some rank, nothing behind it has.
 __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamParams p) {
   __shared__ double lse[NSSM_MAX_BEAMS];
-  __shared__ BeamKey sh[kBeamThreads];
+  __shared__ __align__(16) uint64_t sh[kBeamThreads];
   __shared__ BeamKey cur[kMaxOut], list[kBlock + kMaxOut];
-  __shared__ BeamKey nth;
+  __shared__ uint64_t nth;
   __shared__ int count;
   const int bi = blockIdx.x, tid = threadIdx.x;
   for (int k = tid >> 5; k < p.K; k += kBeamThreads / 32) {   // a warp per beam
@@ -223,7 +305,8 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamPara
   const int64_t all = (int64_t)lists * per;
   int have = 0, quiet = 0;   // entries of cur; candidates since the last one that counted
   for (int64_t c0 = 0; c0 < all && quiet < lists; c0 += kBlock) {
-    BeamKey key[4], best{0, (uint64_t)tid};
+    BeamKey key[4];
+    uint64_t best = 0;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       key[u] = BeamKey{0, 0};
@@ -248,14 +331,15 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamPara
       key[u].hi = order64(total);
       key[u].lo = ((uint64_t)((1 << kBeamBits) - 1 - k) << (32 + kTokenBits)) | ((uint64_t)order32(x) << kTokenBits) |
                   (~tok & ((1u << kTokenBits) - 1));
-      if (best < key[u]) best = key[u];
+      best = key[u].hi > best ? key[u].hi : best;
     }
     if (tid == 0) count = 0;
-    BeamKey tau;
+    // at first the nout-th largest of the threads' best totals: a lower bound
+    BeamKey tau{0, 0};
     if (c0 == 0)
-      tau = nth_of_block<BeamKey>(best, p.n, sh, &nth);
-    else
-      tau = have == p.n ? cur[p.n - 1] : BeamKey{0, 0};
+      tau.hi = nth_of_block(best, p.n, sh, &nth);
+    else if (have == p.n)
+      tau = cur[p.n - 1];
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < 4; ++u)
@@ -297,9 +381,14 @@ namespace {
 
 using nssm_host::fail;
 
-int segments(int V, int bf16) {
-  const int seg = nssm::kBeamThreads * nssm::kVecs * (bf16 ? 8 : 4);
-  return (int)(((int64_t)V + (bf16 ? 7 : 3) + seg - 1) / seg);   // a row may begin inside its first piece
+// CTAs of a row: enough for six waves of the call's CTAs over the SMs (four fit on one), as few as
+// that allows, since every one leaves nout candidates to the merge.
+void row_parts(int64_t rows, int V, int bf16, int* splits, int* steps) {
+  const int per = nssm::kBeamThreads * nssm::kVecs * (bf16 ? 8 : 4);
+  const int all = (int)(((int64_t)V + (bf16 ? 7 : 3) + per - 1) / per);   // a row may begin inside its first piece
+  const int64_t want = (148 * 4 * 6 + rows - 1) / rows;
+  *steps = want >= all ? 1 : (int)((all + want - 1) / want);
+  *splits = (all + *steps - 1) / *steps;
 }
 size_t part_bytes(int64_t rows, int splits) { return ((size_t)rows * splits * sizeof(float2) + 255) / 256 * 256; }
 
@@ -311,8 +400,9 @@ size_t nssm_sizeof_beam_args(void) { return sizeof(nssm_beam_args); }
 
 size_t nssm_beam_workspace_bytes(int32_t batch, int32_t beams, int32_t vocab, int32_t nout, int32_t logits_dtype) {
   if (batch <= 0 || beams <= 0 || vocab <= 0 || nout <= 0) return 0;
-  const int splits = segments(vocab, logits_dtype == NSSM_BF16);
   const int64_t rows = (int64_t)batch * beams;
+  int splits, steps;
+  row_parts(rows, vocab, logits_dtype == NSSM_BF16, &splits, &steps);
   return part_bytes(rows, splits) + (size_t)rows * splits * nout * sizeof(uint64_t);
 }
 
@@ -338,8 +428,8 @@ int nssm_beam_select(const nssm_beam_args* a, void* stream) {
     return fail(NSSM_ERR_INVALID, "a 16-byte aligned workspace of %zu bytes is needed (got %zu)", need, a->workspace_bytes);
   nssm::BeamParams p{};
   p.b = a->batch; p.K = a->beams; p.V = a->vocab; p.n = a->nout; p.eos = a->eos_token;
-  p.bf16 = a->logits_dtype == NSSM_BF16;
-  p.splits = segments(p.V, p.bf16);
+  const int bf16 = a->logits_dtype == NSSM_BF16;
+  row_parts(rows, p.V, bf16, &p.splits, &p.steps);
   p.logits = a->logits; p.l_b = a->logits_stride_b; p.l_k = a->logits_stride_k;
   p.scores = a->scores; p.fin = a->finished;
   p.out_s = a->out_scores; p.out_p = a->out_parents; p.out_t = a->out_tokens; p.out_f = a->out_finished;
@@ -347,7 +437,7 @@ int nssm_beam_select(const nssm_beam_args* a, void* stream) {
   p.cand = reinterpret_cast<uint64_t*>(static_cast<char*>(a->workspace) + part_bytes(rows, p.splits));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid(p.splits, (unsigned)rows);
-  if (p.bf16)
+  if (bf16)
     nssm::beam_scan_kernel<true><<<grid, nssm::kBeamThreads, 0, st>>>(p);
   else
     nssm::beam_scan_kernel<false><<<grid, nssm::kBeamThreads, 0, st>>>(p);

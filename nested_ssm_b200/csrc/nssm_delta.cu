@@ -28,11 +28,15 @@ int check_dims(int H, int G, int P, int N) {
   return NSSM_OK;
 }
 
-// State rows of one head over CTAs: slices of at most 40 rows (8 threads each), so that small
-// batches still spread over the SMs; 40 rather than 32 takes headdim 80 in two slices.
-void slices(int P, int* ns, int* rows) {
-  *ns = (P + 39) / 40;
-  *rows = ((P + *ns - 1) / *ns + 3) / 4 * 4;
+// State rows of one head over CTAs of 4 threads a row: at most 80 rows, and 16 where the whole
+// call would otherwise not give every SM two CTAs.
+void slices(int P, int64_t heads, int* ns, int* rows) {
+  *ns = (P + 79) / 80;
+  *rows = ((P + *ns - 1) / *ns + 7) / 8 * 8;
+  if (heads * *ns < 2 * 148) {
+    *ns = P / 16;
+    *rows = 16;
+  }
 }
 
 using nssm::kC;
@@ -92,7 +96,7 @@ int nssm_delta_step(const nssm_delta_step_args* a, void* stream) {
     return fail(NSSM_ERR_INVALID, "state_stride_s smaller than a slot");
   nssm::DeltaStepParams p{};
   p.H = a->nheads; p.G = a->ngroups; p.P = a->headdim; p.S = a->num_slots;
-  slices(p.P, &p.ns, &p.rows);
+  slices(p.P, (int64_t)a->batch * p.H, &p.ns, &p.rows);
   p.pad = a->pad_slot_id;
   p.io_bf16 = a->io_dtype == NSSM_BF16; p.g_bf16 = a->g_dtype == NSSM_BF16;
   p.beta_bf16 = a->beta_dtype == NSSM_BF16; p.out_bf16 = a->out_dtype == NSSM_BF16;
@@ -111,9 +115,9 @@ int nssm_delta_step(const nssm_delta_step_args* a, void* stream) {
   const dim3 grid(p.H * p.ns, a->batch);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (a->dstate == 64)
-    nssm::delta_step_kernel<64><<<grid, p.rows * 8, 0, st>>>(p);
+    nssm::delta_step_kernel<64><<<grid, p.rows * 4, 0, st>>>(p);
   else
-    nssm::delta_step_kernel<128><<<grid, p.rows * 8, 0, st>>>(p);
+    nssm::delta_step_kernel<128><<<grid, p.rows * 4, 0, st>>>(p);
   return launched("delta_step_kernel");
 }
 

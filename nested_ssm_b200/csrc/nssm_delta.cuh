@@ -52,23 +52,25 @@ __device__ __forceinline__ float4 dl_ld4(const void* p, int64_t i, int bf16, int
 __device__ __forceinline__ float dot4(float4 a, float4 b, float acc) {
   return fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, acc))));
 }
-// sum over the 8 lanes that share a state row
-__device__ __forceinline__ float sum8(float v) {
+// sum over the 4 lanes that share a state row
+__device__ __forceinline__ float sum4(float v) {
   v += __shfl_xor_sync(0xffffffffu, v, 1);
-  v += __shfl_xor_sync(0xffffffffu, v, 2);
-  return v + __shfl_xor_sync(0xffffffffu, v, 4);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
 
-// One decode token.  A CTA takes `rows` state rows of one (batch row, head); 8 lanes share a state
-// row, each with N/32 16-byte pieces of it, so both dot products of a row reduce in 3 shuffles.
-// The output is read off the old state, y = scale (e^g S q + u (k.q)), so that S k and S q reduce
-// together and the row is touched once.
+// One decode token.  A CTA takes `rows` state rows of one (batch row, head); 4 lanes share a state
+// row, each with N/16 16-byte pieces of it in flight at once (128 bytes a thread at N = 128, which
+// is what keeps HBM busy).  k and q of the head wait in shared memory.  The output is read off the
+// old state, y = scale (e^g S q + u (k.q)), so that S k and S q reduce together and the state is
+// read once and written once.
+constexpr int kStepThreads = 320;
 template <int N>
-__global__ void __launch_bounds__(320) delta_step_kernel(const DeltaStepParams p) {
-  constexpr int V = N / 32;
+__global__ void __launch_bounds__(kStepThreads, N == 64 ? 3 : 2) delta_step_kernel(const DeltaStepParams p) {
+  constexpr int V = N / 16;
+  __shared__ float4 sk[N / 4], sq[N / 4];
   const int b = blockIdx.y, h = blockIdx.x / p.ns, slice = blockIdx.x - h * p.ns;
-  const int tid = threadIdx.x, l8 = tid & 7;
-  const int r = slice * p.rows + (tid >> 3);
+  const int tid = threadIdx.x, l4 = tid & 3;
+  const int r = slice * p.rows + (tid >> 2);
   const int slot = p.idx ? p.idx[b] : b;
   if (slot == p.pad) return;
   if (slot < 0 || slot >= p.S) {
@@ -76,46 +78,49 @@ __global__ void __launch_bounds__(320) delta_step_kernel(const DeltaStepParams p
     return;
   }
   const bool live = r < p.P;
-  float* row = p.state + (int64_t)slot * p.st_s + ((int64_t)h * p.P + (live ? r : 0)) * N;
-  float4 s[V], kk[V], qq[V];
+  float4* row = reinterpret_cast<float4*>(p.state + (int64_t)slot * p.st_s + ((int64_t)h * p.P + (live ? r : 0)) * N) + l4;
+  float4 s[V];
 #pragma unroll
-  for (int c = 0; c < V; ++c) s[c] = reinterpret_cast<const float4*>(row)[l8 + 8 * c];
-  // the first row that names a slot owns it
-  int dup = 0;
-  if (p.idx)
-    for (int i = tid; i < b; i += blockDim.x) dup |= p.idx[i] == slot;
+  for (int c = 0; c < V; ++c) s[c] = __ldcs(row + 4 * c);
   const int kh = h / (p.H / p.G);
-#pragma unroll
-  for (int c = 0; c < V; ++c) {
-    const int n = 4 * (l8 + 8 * c);
-    kk[c] = dl_ld4(p.k, b * p.k_b + kh * p.k_h + n, p.io_bf16, p.vec);
-    qq[c] = dl_ld4(p.q, b * p.q_b + kh * p.q_h + n, p.io_bf16, p.vec);
+  for (int i = tid; i < N / 2; i += blockDim.x) {
+    const int n = i & (N / 4 - 1);
+    if (i < N / 4)
+      sk[n] = dl_ld4(p.k, b * p.k_b + kh * p.k_h + 4 * n, p.io_bf16, p.vec);
+    else
+      sq[n] = dl_ld4(p.q, b * p.q_b + kh * p.q_h + 4 * n, p.io_bf16, p.vec);
   }
   const float eg = expf(dl_ld(p.g, b * p.g_b + h * p.g_h, p.g_bf16));
   const float beta = dl_ld(p.beta, b * p.beta_b + h * p.beta_h, p.beta_bf16);
   const float v = live ? dl_ld(p.v, b * p.v_b + h * p.v_h + r, p.io_bf16) : 0.0f;
-  float sk = 0.0f, sq = 0.0f, kq = 0.0f;
-#pragma unroll
-  for (int c = 0; c < V; ++c) {
-    s[c].x *= eg; s[c].y *= eg; s[c].z *= eg; s[c].w *= eg;
-    sk = dot4(s[c], kk[c], sk);
-    sq = dot4(s[c], qq[c], sq);
-    kq = dot4(kk[c], qq[c], kq);
-  }
-  sk = sum8(sk); sq = sum8(sq); kq = sum8(kq);
-  const float u = beta * (v - sk);
+  // the first row that names a slot owns it
+  int dup = 0;
+  if (p.idx)
+    for (int i = tid; i < b; i += blockDim.x) dup |= p.idx[i] == slot;
   if (__syncthreads_or(dup)) {
     if (p.status && blockIdx.x == 0 && tid == 0) atomicOr(p.status, STATUS_CONFLICT);
     return;
   }
+  float ks = 0.0f, qs = 0.0f, kq = 0.0f;
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    const float4 k4 = sk[l4 + 4 * c], q4 = sq[l4 + 4 * c];
+    s[c].x *= eg; s[c].y *= eg; s[c].z *= eg; s[c].w *= eg;
+    ks = dot4(s[c], k4, ks);
+    qs = dot4(s[c], q4, qs);
+    kq = dot4(k4, q4, kq);
+  }
+  ks = sum4(ks); qs = sum4(qs); kq = sum4(kq);
+  const float u = beta * (v - ks);
   if (!live) return;
 #pragma unroll
   for (int c = 0; c < V; ++c) {
-    s[c].x = fmaf(u, kk[c].x, s[c].x); s[c].y = fmaf(u, kk[c].y, s[c].y);
-    s[c].z = fmaf(u, kk[c].z, s[c].z); s[c].w = fmaf(u, kk[c].w, s[c].w);
-    reinterpret_cast<float4*>(row)[l8 + 8 * c] = s[c];
+    const float4 k4 = sk[l4 + 4 * c];
+    s[c].x = fmaf(u, k4.x, s[c].x); s[c].y = fmaf(u, k4.y, s[c].y);
+    s[c].z = fmaf(u, k4.z, s[c].z); s[c].w = fmaf(u, k4.w, s[c].w);
+    __stcs(row + 4 * c, s[c]);
   }
-  if (l8 == 0) dl_st(p.out, b * p.o_b + h * p.o_h + r, p.out_bf16, p.scale * fmaf(u, kq, sq));
+  if (l4 == 0) dl_st(p.out, b * p.o_b + h * p.o_h + r, p.out_bf16, p.scale * fmaf(u, kq, qs));
 }
 
 struct DeltaScanParams {

@@ -14,9 +14,10 @@ namespace nssm {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kMaxRows = NSSM_MAX_SLOT_ROWS;
-constexpr int kRowsPer = kMaxRows / kPlanThreads;   // consecutive rows of one plan thread
 constexpr int kCopyThreads = 256;
 constexpr int kPiece = 32768;                        // bytes of one copy work item
+// Up to these sizes every CTA of the copy makes the plan itself: it costs less than a launch
+constexpr int kFusedRows = 512, kFusedSlots = 16384;
 
 enum : int { STATUS_BAD_SLOT_BIT = 1, STATUS_CONFLICT = NSSM_STATUS_CONFLICT };
 enum : int { PLAN_COPY = 0, PLAN_CLEAR = 1, PLAN_REORDER = 2, PLAN_COMPACT = 3 };
@@ -32,6 +33,7 @@ struct PlanParams {
 };
 
 // Exclusive prefix sum over the CTA of two counts packed in one word each; returns the totals.
+template <int NT>
 __device__ __forceinline__ int2 block_scan2(int2 v, int2* total, int2* warp_sums) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   int2 x = v;
@@ -44,16 +46,16 @@ __device__ __forceinline__ int2 block_scan2(int2 v, int2* total, int2* warp_sums
   if (lane == 31) warp_sums[w] = x;
   __syncthreads();
   if (w == 0) {
-    int2 s = warp_sums[lane];
+    int2 s = lane < NT / 32 ? warp_sums[lane] : make_int2(0, 0);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int yx = __shfl_up_sync(0xffffffffu, s.x, o), yy = __shfl_up_sync(0xffffffffu, s.y, o);
       if (lane >= o) { s.x += yx; s.y += yy; }
     }
-    warp_sums[lane] = s;
+    if (lane < NT / 32) warp_sums[lane] = s;
   }
   __syncthreads();
-  *total = warp_sums[31];
+  *total = warp_sums[NT / 32 - 1];
   const int2 base = w ? warp_sums[w - 1] : make_int2(0, 0);
   return make_int2(base.x + x.x - v.x, base.y + x.y - v.y);
 }
@@ -62,18 +64,20 @@ __device__ __forceinline__ bool bit_set(uint32_t* m, int i) { return (m[i >> 5] 
 
 // The moves of one request.  Dynamic shared memory: three bitmaps over the slots (slots read,
 // slots written, slots written twice), for reorder and compact also two words per row.
-__global__ void __launch_bounds__(kPlanThreads) slot_plan_kernel(const PlanParams p) {
-  extern __shared__ uint32_t sm[];
+// NT threads, kRowsPer consecutive rows each; `count` and `list` receive the moves, the CTA with
+// `lead` also writes new_slots and the status.
+template <int NT, int kRowsPer>
+__device__ __forceinline__ void make_plan(const PlanParams& p, uint32_t* sm, int* count, int2* list, bool lead) {
   __shared__ int2 warp_sums[32];
   __shared__ int err;
   const int words = (p.S + 31) >> 5;
   uint32_t *rd = sm, *wr = sm + words, *wr2 = sm + 2 * words;
   int32_t* first = reinterpret_cast<int32_t*>(sm + 3 * words);   // reorder: first child; both: free slots
   int32_t* freed = first + p.n;
-  for (int i = threadIdx.x; i < 3 * words; i += kPlanThreads) sm[i] = 0;
+  for (int i = threadIdx.x; i < 3 * words; i += NT) sm[i] = 0;
   if (threadIdx.x == 0) err = 0;
   if (p.kind == PLAN_REORDER)
-    for (int i = threadIdx.x; i < p.n; i += kPlanThreads) first[i] = 0x7fffffff;
+    for (int i = threadIdx.x; i < p.n; i += NT) first[i] = 0x7fffffff;
   __syncthreads();
   const int r0 = threadIdx.x * kRowsPer;
   int src[kRowsPer], dst[kRowsPer];   // -1: no move
@@ -118,7 +122,7 @@ __global__ void __launch_bounds__(kPlanThreads) slot_plan_kernel(const PlanParam
       free_row[j] = r < p.n && s != p.pad && s >= 0 && s < p.S && first[r] == 0x7fffffff;
       cnt.x += extra[j]; cnt.y += free_row[j];
     }
-    int2 at = block_scan2(cnt, &total, warp_sums);
+    int2 at = block_scan2<NT>(cnt, &total, warp_sums);
     const int nfree = total.y;
 #pragma unroll
     for (int j = 0; j < kRowsPer; ++j)
@@ -140,7 +144,7 @@ __global__ void __launch_bounds__(kPlanThreads) slot_plan_kernel(const PlanParam
         }
         ++at.x;
       }
-      p.out[r] = s;
+      if (lead) p.out[r] = s;
     }
   } else {
     int2 cnt = make_int2(0, 0);   // x: live rows
@@ -156,7 +160,7 @@ __global__ void __launch_bounds__(kPlanThreads) slot_plan_kernel(const PlanParam
         if (old & (1u << (slot[j] & 31))) bad |= STATUS_CONFLICT;
       }
     }
-    block_scan2(cnt, &total, warp_sums);
+    block_scan2<NT>(cnt, &total, warp_sums);
     const int m = total.x;         // the live slots go to [0, m)
     cnt = make_int2(0, 0);         // x: rows that move, y: free slots below m
 #pragma unroll
@@ -164,12 +168,12 @@ __global__ void __launch_bounds__(kPlanThreads) slot_plan_kernel(const PlanParam
       cnt.x += slot[j] != p.pad && slot[j] >= m;
       cnt.y += r0 + j < m && !bit_set(rd, r0 + j);
     }
-    int2 at = block_scan2(cnt, &total, warp_sums);
+    int2 at = block_scan2<NT>(cnt, &total, warp_sums);
 #pragma unroll
     for (int j = 0; j < kRowsPer; ++j)
       if (r0 + j < m && !bit_set(rd, r0 + j)) freed[at.y++] = r0 + j;
     __syncthreads();
-    for (int i = threadIdx.x; i < words; i += kPlanThreads) rd[i] = 0;
+    for (int i = threadIdx.x; i < words; i += NT) rd[i] = 0;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kRowsPer; ++j) {
@@ -179,7 +183,7 @@ __global__ void __launch_bounds__(kPlanThreads) slot_plan_kernel(const PlanParam
         src[j] = slot[j];
         slot[j] = dst[j] = freed[at.x++];
       }
-      p.out[r0 + j] = slot[j];
+      if (lead) p.out[r0 + j] = slot[j];
     }
   }
 
@@ -204,14 +208,19 @@ __global__ void __launch_bounds__(kPlanThreads) slot_plan_kernel(const PlanParam
         ++cnt.x;
       }
     }
-  int2 at = block_scan2(cnt, &total, warp_sums);
+  int2 at = block_scan2<NT>(cnt, &total, warp_sums);
 #pragma unroll
   for (int j = 0; j < kRowsPer; ++j)
-    if (dst[j] >= 0) p.list[at.x++] = make_int2(src[j], dst[j]);
-  if (threadIdx.x == 0) *p.count = total.x;
+    if (dst[j] >= 0) list[at.x++] = make_int2(src[j], dst[j]);
+  if (threadIdx.x == 0) *count = total.x;
   if (bad) atomicOr(&err, bad);
   __syncthreads();
-  if (threadIdx.x == 0 && err && p.status) atomicOr(p.status, err);
+  if (lead && threadIdx.x == 0 && err && p.status) atomicOr(p.status, err);
+}
+
+__global__ void __launch_bounds__(kPlanThreads) slot_plan_kernel(const PlanParams p) {
+  extern __shared__ __align__(16) uint32_t sm[];
+  make_plan<kPlanThreads, kMaxRows / kPlanThreads>(p, sm, p.count, p.list, true);
 }
 
 struct CopyBuffer {
@@ -252,9 +261,9 @@ __device__ __forceinline__ void copy_piece(char* dst, const char* src, int bytes
   }
 }
 
-__global__ void __launch_bounds__(kCopyThreads) slot_copy_kernel(const CopyParams p) {
+__device__ __forceinline__ void copy_moves(const CopyParams& p, int count, const int2* list) {
   const int pieces = p.buf[p.nbuf - 1].end;
-  const int64_t work = (int64_t)*p.count * pieces;
+  const int64_t work = (int64_t)count * pieces;
   for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
     const int move = (int)(w / pieces);
     int piece = (int)(w - (int64_t)move * pieces), j = 0;
@@ -264,7 +273,7 @@ __global__ void __launch_bounds__(kCopyThreads) slot_copy_kernel(const CopyParam
     const int layer = piece / b.per_row;
     const int64_t off = (int64_t)(piece - layer * b.per_row) * kPiece;
     const int bytes = (int)min((int64_t)kPiece, b.row_bytes - off);
-    const int2 m = p.list[move];
+    const int2 m = list[move];
     const char* src = b.base + layer * b.outer_stride + m.x * b.slot_stride + off;
     char* dst = b.base + layer * b.outer_stride + m.y * b.slot_stride + off;
     if (b.vec == 16)
@@ -274,6 +283,19 @@ __global__ void __launch_bounds__(kCopyThreads) slot_copy_kernel(const CopyParam
     else
       copy_piece<char>(dst, src, bytes, p.clear);
   }
+}
+
+__global__ void __launch_bounds__(kCopyThreads) slot_copy_kernel(const CopyParams p) { copy_moves(p, *p.count, p.list); }
+
+// Plan and copy in one launch.  Every CTA reads the request before it copies and none writes it
+// (new_slots is another array, the leading CTA's alone).
+__global__ void __launch_bounds__(kCopyThreads) slot_move_kernel(const PlanParams q, const CopyParams p) {
+  extern __shared__ __align__(16) uint32_t sm[];
+  __shared__ int2 list[kFusedRows];
+  __shared__ int count;
+  make_plan<kCopyThreads, kFusedRows / kCopyThreads>(q, sm, &count, list, blockIdx.x == 0);
+  __syncthreads();
+  copy_moves(p, count, list);
 }
 
 }  // namespace nssm
@@ -325,19 +347,24 @@ int move(nssm::PlanParams p, const nssm_slot_buffer* bufs, int nbuf, void* ws, s
   const int smem = 3 * ((p.S + 31) / 32) * 4 + 2 * p.n * 4;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e == cudaSuccess && smem > 40 * 1024)
+  const bool fused = p.n <= nssm::kFusedRows && p.S <= nssm::kFusedSlots;
+  if (e == cudaSuccess && !fused && smem > 40 * 1024)
     e = cudaFuncSetAttribute(nssm::slot_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              3 * NSSM_MAX_MOVE_SLOTS / 8 + 2 * NSSM_MAX_SLOT_ROWS * 4);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(NSSM_ERR_CUDA, "slot moves: %s", cudaGetErrorString(e));
   }
-  nssm::slot_plan_kernel<<<1, nssm::kPlanThreads, smem, st>>>(p);
-  if ((e = cudaGetLastError()) != cudaSuccess) return fail(NSSM_ERR_CUDA, "slot_plan_kernel launch: %s", cudaGetErrorString(e));
   const int64_t work = (int64_t)p.n * c.buf[nbuf - 1].end;
   const int grid = (int)(work < 8 * sms ? work : 8 * sms);   // 2048 threads per SM
-  nssm::slot_copy_kernel<<<grid, nssm::kCopyThreads, 0, st>>>(c);
-  if ((e = cudaGetLastError()) != cudaSuccess) return fail(NSSM_ERR_CUDA, "slot_copy_kernel launch: %s", cudaGetErrorString(e));
+  if (fused) {
+    nssm::slot_move_kernel<<<grid, nssm::kCopyThreads, smem, st>>>(p, c);
+  } else {
+    nssm::slot_plan_kernel<<<1, nssm::kPlanThreads, smem, st>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess) return fail(NSSM_ERR_CUDA, "slot_plan_kernel launch: %s", cudaGetErrorString(e));
+    nssm::slot_copy_kernel<<<grid, nssm::kCopyThreads, 0, st>>>(c);
+  }
+  if ((e = cudaGetLastError()) != cudaSuccess) return fail(NSSM_ERR_CUDA, "slot move launch: %s", cudaGetErrorString(e));
   return NSSM_OK;
 }
 
@@ -377,6 +404,7 @@ int nssm_slot_compact(const nssm_slot_buffer* bufs, int32_t nbuf, int32_t num_sl
                       int32_t rows, int32_t pad_slot_id, int32_t* new_slots, void* workspace, size_t workspace_bytes,
                       int32_t* status, void* stream) {
   if (rows > 0 && (!slots || !new_slots)) return fail(NSSM_ERR_INVALID, "slots/new_slots must be non-NULL");
+  if (rows > 0 && new_slots == slots) return fail(NSSM_ERR_INVALID, "new_slots must not be slots");
   nssm::PlanParams p{};
   p.kind = nssm::PLAN_COMPACT;
   p.n = rows; p.S = num_slots; p.pad = pad_slot_id; p.group = 1;

@@ -14,31 +14,33 @@ CUDA device; work is enqueued on that device's current stream and never synchron
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
 from . import _lib
-from .ops import _ptr, _require_cuda, _stream
 from .pool import nssm_dtype
 
 _IO = (torch.bfloat16, torch.float32)
+_pack_step = _lib.packer(_lib.NssmDeltaStepArgs)
+_pack_scan = _lib.packer(_lib.NssmDeltaScanArgs)
 
 
 def _no_grad(*ts):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise RuntimeError("no backward pass: call under torch.no_grad() or detach the inputs")
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("no backward pass: call under torch.no_grad() or detach the inputs")
 
 
 def _check_status(status):
-    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
+    if status.dtype != torch.int32 or status.numel() < 1:
         raise ValueError("status must be an int32 tensor")
 
 
 def _indices(idx, n, name):
-    idx = idx.reshape(-1)
-    if idx.numel() != n:
-        raise ValueError(f"{name} has {idx.numel()} entries, expected {n}")
+    if idx.dim() != 1:
+        idx = idx.reshape(-1)
+    if idx.shape[0] != n:
+        raise ValueError(f"{name} has {idx.shape[0]} entries, expected {n}")
     if idx.dtype != torch.int32 or not idx.is_contiguous():
         idx = idx.to(torch.int32).contiguous()
     return idx
@@ -58,40 +60,43 @@ def gated_delta_state_update(state: torch.Tensor, q, k, v, g, beta, scale: float
     if state.dim() != 4 or state.dtype != torch.float32:
         raise ValueError(f"state must be an fp32 [S, H, P, N] tensor, got {tuple(state.shape)} {state.dtype}")
     S, H, P, N = state.shape
-    if state.stride()[1:] != (P * N, N, 1):
+    ss = state.stride()
+    if ss[1:] != (P * N, N, 1):
         raise ValueError("the heads of a slot must be contiguous in state")
-    if q.dim() != 3 or k.shape != q.shape or q.shape[2] != N:
+    qs = q.shape
+    if len(qs) != 3 or k.shape != qs or qs[2] != N:
         raise ValueError(f"q and k must be [b, G, {N}], got {tuple(q.shape)} and {tuple(k.shape)}")
-    b, G = q.shape[:2]
+    b, G, _ = qs
     if v.shape != (b, H, P) or g.shape != (b, H) or beta.shape != (b, H):
         raise ValueError(f"v must be [{b}, {H}, {P}], g and beta [{b}, {H}], got {tuple(v.shape)}, {tuple(g.shape)}, "
                          f"{tuple(beta.shape)}")
-    if q.dtype not in _IO or k.dtype != q.dtype or v.dtype != q.dtype:
+    dt = q.dtype
+    if dt not in _IO or k.dtype != dt or v.dtype != dt:
         raise ValueError("q, k and v must share a bf16 / fp32 dtype")
     _no_grad(state, q, k, v, g, beta)
-    if q.stride(2) != 1:
-        q = q.contiguous()
-    if k.stride(2) != 1:
-        k = k.contiguous()
-    if v.stride(2) != 1:
-        v = v.contiguous()
+    q0, q1, q2 = q.stride()
+    k0, k1, k2 = k.stride()
+    v0, v1, v2 = v.stride()
+    if q2 != 1 or k2 != 1 or v2 != 1:
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+        (q0, q1, _), (k0, k1, _), (v0, v1, _) = q.stride(), k.stride(), v.stride()
     idx = None if state_batch_indices is None else _indices(state_batch_indices, b, "state_batch_indices")
-    _check_status(status)
+    if status is not None:
+        _check_status(status)
     if out is None:
-        out = torch.empty(b, H, P, dtype=q.dtype, device=state.device)
+        out = torch.empty(b, H, P, dtype=dt, device=state.device)
     elif out.shape != (b, H, P) or out.stride(2) != 1 or out.dtype not in _IO:
         raise ValueError(f"out must be [{b}, {H}, {P}] bf16 / fp32 with unit inner stride")
-    dev = _require_cuda(state, q, k, v, g, beta, idx, out, status)
-    a = _lib.NssmDeltaStepArgs(
-        b, S, H, G, P, N, nssm_dtype(q.dtype), nssm_dtype(g.dtype), nssm_dtype(beta.dtype), nssm_dtype(out.dtype),
-        int(pad_slot_id), N ** -0.5 if scale is None else float(scale),
-        state.data_ptr(), state.stride(0), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
-        k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), g.data_ptr(), g.stride(0), g.stride(1),
-        beta.data_ptr(), beta.stride(0), beta.stride(1), _ptr(idx), out.data_ptr(), out.stride(0), out.stride(1),
-        _ptr(status))
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        _lib.check(lib.nssm_delta_step(C.byref(a), _stream(dev)))
+    dev = _lib.device_index(state, q, k, v, g, beta, idx, out, status)
+    o0, o1, _ = out.stride()
+    g0, g1 = g.stride()
+    b0, b1 = beta.stride()
+    a = _pack_step(
+        b, S, H, G, P, N, nssm_dtype(dt), nssm_dtype(g.dtype), nssm_dtype(beta.dtype), nssm_dtype(out.dtype),
+        int(pad_slot_id), N ** -0.5 if scale is None else float(scale), state.data_ptr(), ss[0], q.data_ptr(), q0, q1,
+        k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, g.data_ptr(), g0, g1, beta.data_ptr(), b0, b1,
+        0 if idx is None else idx.data_ptr(), out.data_ptr(), o0, o1, 0 if status is None else status.data_ptr())
+    _lib.call(_lib.load().nssm_delta_step, dev, a)
     return out
 
 
@@ -159,19 +164,18 @@ def gated_delta_chunk_scan(q, k, v, g, beta, scale: float | None = None, initial
             raise ValueError(f"final_states must be fp32 [{n}, {H}, {P}, {N}] with contiguous rows")
     elif return_final_states:
         final_states = torch.empty(n, H, P, N, dtype=torch.float32, device=q.device)
-    _check_status(status)
-    dev = _require_cuda(q, k, v, g, beta, cu_seqlens, initial_states, out, final_states, status)
+    if status is not None:
+        _check_status(status)
+    dev = _lib.device_index(q, k, v, g, beta, cu_seqlens, initial_states, out, final_states, status)
     lib = _lib.load()
     nbytes = lib.nssm_delta_scan_workspace_bytes(n, T, H, G, N, int(cu_seqlens is not None))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    a = _lib.NssmDeltaScanArgs(
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    a = _pack_scan(
         n, T, H, G, P, N, nssm_dtype(g.dtype), nssm_dtype(beta.dtype), N ** -0.5 if scale is None else float(scale), 0,
-        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-        v.data_ptr(), v.stride(0), v.stride(1), g.data_ptr(), g.stride(0), g.stride(1),
-        beta.data_ptr(), beta.stride(0), beta.stride(1), _ptr(cu_seqlens),
-        _ptr(initial_states), initial_states.stride(0) if initial_states is not None else 0,
-        out.data_ptr(), out.stride(0), out.stride(1),
-        _ptr(final_states), final_states.stride(0) if final_states is not None else 0, _ptr(ws), nbytes, _ptr(status))
-    with torch.cuda.device(dev):
-        _lib.check(lib.nssm_delta_scan(C.byref(a), _stream(dev)))
+        q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2], g.data_ptr(),
+        *g.stride()[:2], beta.data_ptr(), *beta.stride()[:2], ptr(cu_seqlens),
+        ptr(initial_states), 0 if initial_states is None else initial_states.stride(0), out.data_ptr(), *out.stride()[:2],
+        ptr(final_states), 0 if final_states is None else final_states.stride(0), ptr(ws), nbytes, ptr(status))
+    _lib.call(lib.nssm_delta_scan, dev, a)
     return (out, final_states) if return_final_states else out

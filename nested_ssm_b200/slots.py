@@ -10,12 +10,9 @@ another move reads are dropped, and ``check_status()`` of the buffers raises for
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
 from . import _lib
-from .ops import _ptr, _require_cuda, _stream
 from .pool import TieredSlotPool
 
 
@@ -55,7 +52,8 @@ class StateBuffers:
             raise ValueError(f"{self.num_slots} slots; at most {_lib.MAX_MOVE_SLOTS}")
         self.tensors, self.slot_dim = tensors, slot_dim
         self._bufs = _describe(tensors, slot_dim)
-        self.device = _require_cuda(*tensors)
+        _lib.device_index(*tensors)
+        self.device = tensors[0].device
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
 
     def check_status(self) -> None:
@@ -83,63 +81,57 @@ def _target(buffers):
 
 
 def _list(t, name, n=None):
-    if t.is_floating_point() or t.dtype == torch.bool:
-        raise ValueError(f"{name} must hold integers, got {t.dtype}")
-    f = t.reshape(-1)
-    if n is not None and f.numel() != n:
-        raise ValueError(f"{name} has {f.numel()} entries, expected {n}")
-    if f.numel() > _lib.MAX_SLOT_ROWS:
-        raise ValueError(f"{name} has {f.numel()} rows; at most {_lib.MAX_SLOT_ROWS} in one call")
-    if f.dtype != torch.int32 or not f.is_contiguous():
-        f = f.to(torch.int32).contiguous()
-    return f
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        if t.is_floating_point() or t.dtype == torch.bool:
+            raise ValueError(f"{name} must hold integers, got {t.dtype}")
+        t = t.to(torch.int32).contiguous()
+    rows = t.numel()
+    if n is not None and rows != n:
+        raise ValueError(f"{name} has {rows} entries, expected {n}")
+    if rows > _lib.MAX_SLOT_ROWS:
+        raise ValueError(f"{name} has {rows} rows; at most {_lib.MAX_SLOT_ROWS} in one call")
+    return t
 
 
-def _workspace(n, dev):
-    return torch.empty(8 + 8 * max(n, 1), dtype=torch.uint8, device=dev)
+def _workspace(n, device):
+    return torch.empty(8 + 8 * max(n, 1), dtype=torch.uint8, device=device)
+
+
+def _copy(buffers, src, dst, pad_slot_id):
+    bufs, S, where, status = _target(buffers)
+    n = dst.numel()
+    dev = _lib.device_index(status, src, dst)
+    ws = _workspace(n, where)
+    _lib.call(_lib.load().nssm_slot_copy, dev, bufs, len(bufs), S, None if src is None else src.data_ptr(), dst.data_ptr(),
+              n, int(pad_slot_id), ws.data_ptr(), ws.numel(), status.data_ptr())
 
 
 def copy_slots(buffers, src: torch.Tensor, dst: torch.Tensor, pad_slot_id: int = -1) -> None:
     """Slot ``dst[i]`` becomes a copy of slot ``src[i]``; naming a source several times forks it.
     Pairs with ``pad_slot_id`` are skipped, a pair with ``src == dst`` does nothing."""
-    bufs, S, dev, status = _target(buffers)
-    s = _list(src, "src")
-    d = _list(dst, "dst", s.numel())
-    _require_cuda(s, d, status)
-    ws = _workspace(s.numel(), dev)
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        _lib.check(lib.nssm_slot_copy(bufs, len(bufs), S, s.data_ptr(), d.data_ptr(), s.numel(), int(pad_slot_id),
-                                      ws.data_ptr(), ws.numel(), status.data_ptr(), _stream(dev)))
+    src = _list(src, "src")
+    _copy(buffers, src, _list(dst, "dst", src.numel()), pad_slot_id)
 
 
 def clear_slots(buffers, slots: torch.Tensor, pad_slot_id: int = -1) -> None:
     """Free slots: every value of the named slots becomes zero, an empty state for the next
     sequence."""
-    bufs, S, dev, status = _target(buffers)
-    d = _list(slots, "slots")
-    _require_cuda(d, status)
-    ws = _workspace(d.numel(), dev)
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        _lib.check(lib.nssm_slot_copy(bufs, len(bufs), S, None, d.data_ptr(), d.numel(), int(pad_slot_id),
-                                      ws.data_ptr(), ws.numel(), status.data_ptr(), _stream(dev)))
+    _copy(buffers, None, _list(slots, "slots"), pad_slot_id)
 
 
 def compact_slots(buffers, slots: torch.Tensor, pad_slot_id: int = -1) -> torch.Tensor:
     """Move the m live slots of ``slots`` into slots 0 .. m-1 and return where each row's slot is
     now (int32, ``slots``' shape; padded rows stay padded).  Slots below m stay, the others take the
     free slots below m in row order: the fewest copies."""
-    bufs, S, dev, status = _target(buffers)
+    bufs, S, where, status = _target(buffers)
     s = _list(slots, "slots")
-    _require_cuda(s, status)
-    ws = _workspace(s.numel(), dev)
+    n = s.numel()
+    dev = _lib.device_index(status, s)
+    ws = _workspace(n, where)
     new = torch.empty_like(s)
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        _lib.check(lib.nssm_slot_compact(bufs, len(bufs), S, s.data_ptr(), s.numel(), int(pad_slot_id), new.data_ptr(),
-                                         ws.data_ptr(), ws.numel(), status.data_ptr(), _stream(dev)))
-    return new.view(slots.shape)
+    _lib.call(_lib.load().nssm_slot_compact, dev, bufs, len(bufs), S, s.data_ptr(), n, int(pad_slot_id), new.data_ptr(),
+              ws.data_ptr(), ws.numel(), status.data_ptr())
+    return new
 
 
 def reorder_slots(buffers, slots: torch.Tensor, parents: torch.Tensor, pad_slot_id: int = -1) -> torch.Tensor:
@@ -149,17 +141,16 @@ def reorder_slots(buffers, slots: torch.Tensor, parents: torch.Tensor, pad_slot_
     (:func:`~nested_ssm_b200.beam.beam_select`); 1-D: parents are rows of the whole batch.  The first
     child of a row keeps its slot, every other child takes the slot of a row without children and
     gets a copy of the state there: the fewest copies.  A row whose parent is padded becomes padded."""
-    if parents.shape != slots.shape:
-        raise ValueError(f"parents {tuple(parents.shape)} must have slots' shape {tuple(slots.shape)}")
-    bufs, S, dev, status = _target(buffers)
+    shape = slots.shape
+    if parents.shape != shape:
+        raise ValueError(f"parents {tuple(parents.shape)} must have slots' shape {tuple(shape)}")
+    bufs, S, where, status = _target(buffers)
     s, p = _list(slots, "slots"), _list(parents, "parents")
-    _require_cuda(s, p, status)
     n = s.numel()
-    group = slots.shape[-1] if slots.dim() > 1 else n
-    ws = _workspace(n, dev)
+    dev = _lib.device_index(status, s, p)
+    ws = _workspace(n, where)
     new = torch.empty_like(s)
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        _lib.check(lib.nssm_slot_reorder(bufs, len(bufs), S, s.data_ptr(), p.data_ptr(), n, max(group, 1), int(pad_slot_id),
-                                         new.data_ptr(), ws.data_ptr(), ws.numel(), status.data_ptr(), _stream(dev)))
-    return new.view(slots.shape)
+    _lib.call(_lib.load().nssm_slot_reorder, dev, bufs, len(bufs), S, s.data_ptr(), p.data_ptr(), n,
+              max(shape[-1] if len(shape) > 1 else n, 1), int(pad_slot_id), new.data_ptr(), ws.data_ptr(), ws.numel(),
+              status.data_ptr())
+    return new
