@@ -70,93 +70,188 @@ __device__ __forceinline__ uint64_t nth_of_block(uint64_t mine, int n, uint64_t*
   return *result;
 }
 
-// A part of a row, a step of kBeamThreads * kVecs 16-byte pieces at a time; the max, the sum and
-// the candidates of a step all come from one read into registers.  Only values that reach a lower
-// bound of the nout-th best so far become candidates: at first the nout-th best of a few maxima of
-// each warp, then the nout-th best itself.  Any bound is safe; one that lets through too many
-// (sorted or constant logits) is replaced by the nout-th largest of the threads' own best keys,
-// which lets through at most nout threads' values.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// The pieces of one step of one thread, as fp32 values (-inf outside the row and for what is not
+// finite) with each piece's maximum.
 template <bool BF16>
-__global__ void __launch_bounds__(kBeamThreads, 4) beam_scan_kernel(const BeamParams p) {
-  constexpr int E = BF16 ? 8 : 4;                       // elements of a 16-byte piece
-  constexpr int kStep = kBeamThreads * kVecs * E;
-  constexpr int kCap = kMaxOut * kVecs * E;             // candidates of kMaxOut threads
-  __shared__ __align__(16) uint64_t sh[kBeamThreads];
-  __shared__ uint64_t list[kCap + kMaxOut], cur[kMaxOut];
-  __shared__ float red[kBeamWarps], rsum[kBeamWarps];
-  __shared__ uint64_t nth;
-  __shared__ int count;
-  const int row = blockIdx.y, bi = row / p.K, ki = row - bi * p.K, split = blockIdx.x;
-  if (p.fin && p.fin[row]) return;                      // the merge knows its one candidate
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int es = BF16 ? 2 : 4;
-  const char* base = static_cast<const char*>(p.logits) + (bi * p.l_b + ki * p.l_k) * es;
-  // pieces are 16-byte aligned in memory: piece 0 of the row may begin before the row does
-  const int lead = (int)((reinterpret_cast<uintptr_t>(base) & 15) / es);
-  const int steps = min(p.steps, (p.V + lead + kStep - 1) / kStep - split * p.steps);
-  float m = kNegInf, sum = 0.0f;                        // this thread's running maximum and sum
-  int have = 0;                                         // entries of cur, sorted
-  if (tid == 0) count = 0;
-  for (int st = 0; st < steps; ++st) {
-    const int first = (split * p.steps + st) * kStep + tid * E - lead;
-    float x[kVecs * E];
-    float mx = kNegInf;
-    bool odd = false;
-#pragma unroll
-    for (int c = 0; c < kVecs; ++c) {
-      const int t0 = first + c * kBeamThreads * E;
-      if (t0 >= 0 && t0 + E <= p.V) {
-        const uint4 r = __ldg(reinterpret_cast<const uint4*>(base + (int64_t)t0 * es));
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (BF16) {
-            x[c * E + 2 * i] = __uint_as_float(w[i] << 16);
-            x[c * E + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-          } else {
-            x[c * E + i] = __uint_as_float(w[i]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          const int t = t0 + i;
-          x[c * E + i] = kNegInf;
-          if (t >= 0 && t < p.V)
-            x[c * E + i] = BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[t])
-                                : reinterpret_cast<const float*>(base)[t];
-        }
+struct BeamRow {
+  static constexpr int E = BF16 ? 8 : 4;                // elements of a 16-byte piece
+  static constexpr int kStep = kBeamThreads * kVecs * E;
+  static constexpr int es = BF16 ? 2 : 4;
+  const char* base;
+  int V, lead;    // pieces are 16-byte aligned in memory: piece 0 may begin `lead` elements before the row
+
+  __device__ __forceinline__ int first(int step, int c) const {
+    return step * kStep + (c * kBeamThreads + (int)threadIdx.x) * E - lead;
+  }
+  // a piece that crosses an end of the row, -inf outside
+  static __device__ __noinline__ uint4 edge(const char* base, int V, int t0) {
+    uint32_t w[4];
+#pragma unroll 1
+    for (int q = 0; q < 4; ++q) {
+      uint32_t v = 0;
+#pragma unroll 1
+      for (int i = 0; i < E / 4; ++i) {
+        const int t = t0 + q * (E / 4) + i;
+        const bool in = t >= 0 && t < V;
+        if constexpr (BF16)
+          v |= (in ? (uint32_t) reinterpret_cast<const uint16_t*>(base)[t] : 0xff80u) << (16 * i);
+        else
+          v = in ? reinterpret_cast<const uint32_t*>(base)[t] : 0xff800000u;
       }
+      w[q] = v;
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ void load(int t0, uint4& r) const {
+    r = t0 >= 0 && t0 + E <= V ? __ldg(reinterpret_cast<const uint4*>(base + (int64_t)t0 * es)) : edge(base, V, t0);
+  }
+  __device__ __forceinline__ void fetch(int step, uint4* r) const {
 #pragma unroll
-    for (int i = 0; i < kVecs * E; ++i) {
-      odd |= !(x[i] <= 3.402823466e38f);
-      mx = fmaxf(mx, x[i]);
+    for (int c = 0; c < kVecs; ++c) load(first(step, c), r[c]);
+  }
+  // E values of a piece and the largest
+  static __device__ __forceinline__ void values(const uint4& raw, float* x, float& mx) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    if constexpr (BF16) {
+      __nv_bfloat162 m2 = *reinterpret_cast<const __nv_bfloat162*>(&w[0]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        if (i) m2 = __hmax2_nan(m2, *reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+      }
+      mx = max_nan(__low2float(m2), __high2float(m2));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+      mx = max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3]));
     }
-    if (odd) {       // NaN and +inf count as masked
+    if (!(mx <= 3.402823466e38f)) {              // NaN and +inf count as masked
       mx = kNegInf;
 #pragma unroll
-      for (int i = 0; i < kVecs * E; ++i) {
+      for (int i = 0; i < E; ++i) {
         if (!(x[i] <= 3.402823466e38f)) x[i] = kNegInf;
         mx = fmaxf(mx, x[i]);
       }
     }
+  }
+  static __device__ __forceinline__ float unpack(const uint4* raw, float* x, float* mxc) {
+#pragma unroll
+    for (int c = 0; c < kVecs; ++c) values(raw[c], x + c * E, mxc[c]);
+    return fmaxf(fmaxf(mxc[0], mxc[1]), fmaxf(mxc[2], mxc[3]));
+  }
+};
+
+// The n best of list[0, total) to cur, sorted, by counting for each how many are larger.
+__device__ __forceinline__ int rank_list(const uint64_t* list, int total, int n, uint64_t* cur) {
+  for (int i = threadIdx.x; i < total; i += kBeamThreads) {
+    const uint64_t k = list[i];
+    int rank = 0;
+    for (int j = 0; j < total; ++j) rank += list[j] > k;
+    if (rank < n) cur[rank] = k;
+  }
+  __syncthreads();
+  return min(total, n);
+}
+
+// The part again, exactly: each step's candidates are those above the nout-th largest of the
+// threads' own best keys, at most nout threads' values.
+template <bool BF16>
+__device__ __noinline__ int beam_exact(BeamRow<BF16> r, int step0, int steps, int n, uint64_t* sh, uint64_t* list,
+                                       uint64_t* cur, uint64_t* nth, int* count) {
+  constexpr int E = BeamRow<BF16>::E;
+  int have = 0;
+  for (int st = step0; st < step0 + steps; ++st) {
+    uint4 raw[kVecs];
+    float x[kVecs * E], mxc[kVecs];
+    r.fetch(st, raw);
+    r.unpack(raw, x, mxc);
+    uint64_t best = 0;
+#pragma unroll
+    for (int i = 0; i < kVecs * E; ++i) {
+      const int tk = r.first(st, i / E) + i % E;
+      const uint64_t k = tk >= 0 && tk < r.V ? key_of(x[i], tk) : 0;
+      best = k > best ? k : best;
+    }
+    if (threadIdx.x == 0) *count = 0;
+    const uint64_t least = nth_of_block(best, n, sh, nth);
+    if (best >= least)
+#pragma unroll
+      for (int i = 0; i < kVecs * E; ++i) {
+        const int tk = r.first(st, i / E) + i % E;
+        if (tk >= 0 && tk < r.V && key_of(x[i], tk) >= least) list[atomicAdd(count, 1)] = key_of(x[i], tk);
+      }
+    __syncthreads();
+    const int found = *count;
+    for (int i = threadIdx.x; i < have; i += kBeamThreads) list[found + i] = cur[i];
+    __syncthreads();
+    have = rank_list(list, found + have, n, cur);
+  }
+  return have;
+}
+
+// A part of a row, a step of kBeamThreads * kVecs 16-byte pieces at a time, the next one's loads in
+// flight; the max, the sum and the candidates of a step all come from one read into registers.
+// Candidates are the values that reach a lower bound of the nout-th best, the nout-th best of a
+// few maxima of each warp in the first step, so later steps need no barrier; a step only notes
+// the pieces that hold any, which are read again and ranked at the end.  Where the bound lets
+// through too many (sorted or constant logits), beam_exact reads the part again.
+template <bool BF16>
+__global__ void __launch_bounds__(kBeamThreads, BF16 ? 3 : 4) beam_scan_kernel(const BeamParams p) {
+  using Row = BeamRow<BF16>;
+  constexpr int E = Row::E;
+  constexpr int kCap = kMaxOut * kVecs * E;             // beam_exact's candidates: kMaxOut threads' values
+  constexpr int kPieces = 1024;
+  __shared__ __align__(16) uint64_t sh[kBeamThreads];
+  __shared__ uint64_t list[kCap + kMaxOut], cur[kMaxOut];
+  __shared__ float red[kBeamWarps], rsum[kBeamWarps];
+  __shared__ uint64_t nth;
+  __shared__ int plist[kPieces];                        // first tokens of the pieces that reach the bound
+  __shared__ int count, pieces;
+  const int row = blockIdx.y, bi = row / p.K, ki = row - bi * p.K, split = blockIdx.x;
+  if (p.fin && p.fin[row]) return;                      // the merge knows its one candidate
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  Row r;
+  r.base = static_cast<const char*>(p.logits) + (bi * p.l_b + ki * p.l_k) * Row::es;
+  r.V = p.V;
+  r.lead = (int)((reinterpret_cast<uintptr_t>(r.base) & 15) / Row::es);
+  const int step0 = split * p.steps;
+  const int steps = max(0, min(p.steps, (p.V + r.lead + Row::kStep - 1) / Row::kStep - step0));
+  float m = kNegInf, sum = 0.0f;                        // this thread's running maximum and sum
+  float tau = kNegInf;
+  if (tid == 0) count = pieces = 0;
+  uint4 raw[kVecs];
+  if (steps > 0) r.fetch(step0, raw);
+  for (int st = step0; st < step0 + steps; ++st) {
+    float x[kVecs * E], mxc[kVecs];
+    const float mx = r.unpack(raw, x, mxc);
+    if (st + 1 < step0 + steps) r.fetch(st + 1, raw);
     if (mx > m) {
       sum *= ex2((m - mx) * kLog2e);
       m = mx;
     }
     if (m != kNegInf) {
-      // the difference first: x and m may both be the type's lowest value
-      float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      float2 s2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+      if (fabsf(m) < 1e38f) {
+        const float2 l2 = make_float2(kLog2e, kLog2e), off = make_float2(-m * kLog2e, -m * kLog2e);
 #pragma unroll
-      for (int i = 0; i < kVecs * E; ++i) s4[i & 3] += ex2((x[i] - m) * kLog2e);
-      sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+        for (int i = 0; i < kVecs * E; i += 2) {
+          const float2 e = __ffma2_rn(make_float2(x[i], x[i + 1]), l2, off);
+          s2[(i >> 1) & 1] = __fadd2_rn(s2[(i >> 1) & 1], make_float2(ex2(e.x), ex2(e.y)));
+        }
+      } else {     // near the type's lowest or largest value: the difference first
+#pragma unroll
+        for (int i = 0; i < kVecs * E; ++i) s2[0].x += ex2((x[i] - m) * kLog2e);
+      }
+      sum += (s2[0].x + s2[0].y) + (s2[1].x + s2[1].y);
     }
-    // the bound
-    float tau;
-    if (have == p.n) {
-      tau = unorder32((uint32_t)(cur[p.n - 1] >> 32));
-    } else {
+    if (st == step0) {
       const int t = min(32, (2 * p.n + kBeamWarps - 1) / kBeamWarps);   // maxima of each warp
       uint32_t mine = order32(mx);
       for (int k = 0; k < t; ++k) {
@@ -166,71 +261,45 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_scan_kernel(const BeamPa
         if (lane == who) mine = 0;
       }
       __syncthreads();
-      int rank = 0;
       const uint64_t v = tid < kBeamWarps * t ? sh[tid] : 0;
+      int rank = 0;
       for (int i = 0; i < kBeamWarps * t; ++i) rank += sh[i] > v || (sh[i] == v && i < tid);
       if (tid < kBeamWarps * t && rank == p.n - 1) nth = v;
       __syncthreads();
       tau = unorder32((uint32_t)nth);
-      if (!(tau >= kNegInf)) tau = kNegInf;
+      if (!(tau >= kNegInf)) tau = kNegInf;     // fewer values than that
     }
-    int mycount = 0;
-    if (mx >= tau)
 #pragma unroll
-      for (int i = 0; i < kVecs * E; ++i) {
-        const int tk = first + (i / E) * kBeamThreads * E + i % E;
-        if (x[i] >= tau && tk >= 0 && tk < p.V) ++mycount;
+    for (int c = 0; c < kVecs; ++c)
+      if (mxc[c] >= tau) {
+        const int at = atomicAdd(&pieces, 1);
+        if (at < kPieces) plist[at] = r.first(st, c);
       }
-    int at = mycount ? atomicAdd(&count, mycount) : 0;
-    __syncthreads();
-    int found = count;
-    uint64_t least = 0;
-    const bool many = found > max(256, 4 * p.n);
-    if (many) {
-      uint64_t best = 0;
-#pragma unroll
-      for (int i = 0; i < kVecs * E; ++i) {
-        const int tk = first + (i / E) * kBeamThreads * E + i % E;
-        const uint64_t k = tk >= 0 && tk < p.V ? key_of(x[i], tk) : 0;
-        best = k > best ? k : best;
-      }
-      least = nth_of_block(best, p.n, sh, &nth);
-      mycount = 0;
-      if (best >= least)
-#pragma unroll
-        for (int i = 0; i < kVecs * E; ++i) {
-          const int tk = first + (i / E) * kBeamThreads * E + i % E;
-          if (tk >= 0 && tk < p.V && key_of(x[i], tk) >= least) ++mycount;
-        }
-      if (tid == 0) count = 0;
-      __syncthreads();
-      at = mycount ? atomicAdd(&count, mycount) : 0;
-      __syncthreads();
-      found = count;
-    }
-    if (mycount)
-#pragma unroll
-      for (int i = 0; i < kVecs * E; ++i) {
-        const int tk = first + (i / E) * kBeamThreads * E + i % E;
-        if (tk < 0 || tk >= p.V) continue;
-        if (many ? key_of(x[i], tk) >= least : x[i] >= tau) list[at++] = key_of(x[i], tk);
-      }
-    __syncthreads();     // every thread has read count
-    if (found) {
-      for (int i = tid; i < have; i += kBeamThreads) list[found + i] = cur[i];
-      if (tid == 0) count = 0;
-      __syncthreads();
-      const int total = found + have;
-      for (int i = tid; i < total; i += kBeamThreads) {
-        const uint64_t k = list[i];
-        int rank = 0;
-        for (int j = 0; j < total; ++j) rank += list[j] > k;
-        if (rank < p.n) cur[rank] = k;
-      }
-      have = min(total, p.n);
-      __syncthreads();
-    }
   }
+  __syncthreads();
+  const int np = pieces;
+  if (np <= kPieces)
+    for (int i = tid; i < np; i += kBeamThreads) {   // the values of the few pieces that reach the bound, read again
+      uint4 one;
+      float v[E], top;
+      r.load(plist[i], one);
+      r.values(one, v, top);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int tk = plist[i] + e;
+        if (v[e] >= tau && tk >= 0 && tk < p.V) {
+          const int at = atomicAdd(&count, 1);
+          if (at < kCap) list[at] = key_of(v[e], tk);
+        }
+      }
+    }
+  __syncthreads();
+  // ranking is quadratic in the list: beyond this beam_exact's shorter lists are the cheaper way
+  const int found = count;
+  __syncthreads();
+  const int have = np <= kPieces && found <= max(512, 4 * p.n)
+                       ? rank_list(list, found, p.n, cur)
+                       : beam_exact<BF16>(r, step0, steps, p.n, sh, list, cur, &nth, &count);
   uint64_t* out = p.cand + ((int64_t)row * p.splits + split) * p.n;
   for (int i = tid; i < p.n; i += kBeamThreads) out[i] = i < have ? cur[i] : 0;
   // the part's maximum and sum
@@ -381,12 +450,13 @@ namespace {
 
 using nssm_host::fail;
 
-// CTAs of a row: enough for six waves of the call's CTAs over the SMs (four fit on one), as few as
-// that allows, since every one leaves nout candidates to the merge.
+// CTAs of a row: about two waves of the call's CTAs over the SMs (three fit on one), as few as that
+// allows: a part's first step pays for the bound, and every part leaves nout candidates to the
+// merge (64 x 8 rows of 131072: 48 us with two waves, 54 with four, 68 with six).
 void row_parts(int64_t rows, int V, int bf16, int* splits, int* steps) {
   const int per = nssm::kBeamThreads * nssm::kVecs * (bf16 ? 8 : 4);
   const int all = (int)(((int64_t)V + (bf16 ? 7 : 3) + per - 1) / per);   // a row may begin inside its first piece
-  const int64_t want = (148 * 4 * 6 + rows - 1) / rows;
+  const int64_t want = (148 * 3 * 2 + rows - 1) / rows;
   *steps = want >= all ? 1 : (int)((all + want - 1) / want);
   *splits = (all + *steps - 1) / *steps;
 }
