@@ -50,7 +50,7 @@ int64_t ws_chunks(int batch, int seqlen, int packed) {
 template <int N>
 int launch_chunks(nssm::DeltaChunkParams& p, void* ws, cudaStream_t st) {
   auto prep = nssm::delta_prep_kernel<N>;
-  auto walk = p.s.G * p.tile_groups * p.s.B > 296 ? nssm::delta_chunk_kernel<N, 3> : nssm::delta_chunk_kernel<N, 2>;
+  auto walk = nssm::delta_chunk_kernel<N>;
   p.img = static_cast<unsigned char*>(ws);
   p.blk = p.img + (int64_t)p.chunks * p.s.G * nssm::kImgBytes<N>;
   const int smem = nssm::ChunkSmem<N>::bytes(p.heads);
@@ -62,12 +62,13 @@ int launch_chunks(nssm::DeltaChunkParams& p, void* ws, cudaStream_t st) {
     cudaGetLastError();
     return fail(NSSM_ERR_CUDA, "delta scan: %s", cudaGetErrorString(e));
   }
+  const dim3 grid(p.s.G * p.tile_groups, p.s.B), block(nssm::kWarps * 32);
   if (p.chunks > 0) {
     prep<<<dim3(p.chunks, p.s.G), nssm::kPrepThreads, nssm::PrepSmem<N>::kBytes, st>>>(p);
     const int rc = launched("delta_prep_kernel");
     if (rc) return rc;
   }
-  walk<<<dim3(p.s.G * p.tile_groups, p.s.B), nssm::kWarps * 32, smem, st>>>(p);
+  walk<<<grid, block, smem, st>>>(p);
   return launched("delta_chunk_kernel");
 }
 
@@ -167,8 +168,8 @@ int nssm_delta_scan(const nssm_delta_scan_args* a, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const size_t need = nssm_delta_scan_workspace_bytes(a->batch, a->seqlen, a->nheads, a->ngroups, a->dstate,
                                                     a->cu_seqlens != nullptr);
-  if (need && (!a->workspace || !al(a->workspace, 16) || a->workspace_bytes < need))
-    return fail(NSSM_ERR_INVALID, "a 16-byte aligned workspace of %zu bytes is needed (got %zu)", need, a->workspace_bytes);
+  if (need && (!a->workspace || !al(a->workspace, 32) || a->workspace_bytes < need))
+    return fail(NSSM_ERR_INVALID, "a 32-byte aligned workspace of %zu bytes is needed (got %zu)", need, a->workspace_bytes);
   nssm::DeltaChunkParams c{};
   c.s = p;
   c.chunks = (int)ws_chunks(a->batch, a->seqlen, a->cu_seqlens != nullptr);

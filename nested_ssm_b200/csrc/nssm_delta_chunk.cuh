@@ -41,7 +41,7 @@ __host__ __device__ constexpr int frag_index(int nt, int ks) { return nt < 2 ? n
 // e^{G_C - G} and 1.
 constexpr int kBlkM = 2 * kFrags * kFragBytes;
 constexpr int kBlkF = kBlkM + kFrags * kFragBytes;
-constexpr int kBlkBytes = kBlkF + 5 * kC * 4 + 16;
+constexpr int kBlkBytes = kBlkF + 5 * kC * 4 + 32;    // whole sectors
 // and of a (chunk, group): K^ and Q^ as the walk wants them in shared memory
 template <int N> constexpr int kImgBytes = 2 * kC * N * 2;
 
@@ -111,6 +111,13 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// 32 bytes, a whole sector (two 16-byte stores would each write half of it)
+__device__ __forceinline__ void st32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 
 // Byte offset of 16-byte piece c of row r in a [rows][N] bf16 tile: the pieces of 8 consecutive
 // rows at one column lie in 8 different bank groups.
@@ -299,9 +306,7 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const DeltaChu
         mw[(c & 7) + (c >> 3) + 2] = hf2(m[2], m[3]);
       }
       if (lane >= 16 * ks) {
-        uint4* o = reinterpret_cast<uint4*>(frow + kBlkM + frag_index(lane >> 3, ks) * kFragBytes);
-        o[0] = make_uint4(mw[0], mw[1], mw[2], mw[3]);
-        o[1] = make_uint4(mw[4], mw[5], mw[6], mw[7]);
+        st32(frow + kBlkM + frag_index(lane >> 3, ks) * kFragBytes, mw);
       }
     }
     __syncwarp();
@@ -335,12 +340,8 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const DeltaChu
 #pragma unroll
         for (int c = 0; c < 16; c += 2)
           split2(st.s * x[16 * ks + c], st.s * x[16 * ks + c + 1], hi[(c & 7) + (c >> 3)], lo[(c & 7) + (c >> 3)]);
-        uint4* o = reinterpret_cast<uint4*>(frow + frag_index(lane >> 3, ks) * kFragBytes);
-        o[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        o[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-        o += kFrags * kFragBytes / 16;
-        o[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        o[1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+        st32(frow + frag_index(lane >> 3, ks) * kFragBytes, hi);
+        st32(frow + (kFrags + frag_index(lane >> 3, ks)) * kFragBytes, lo);
       }
     __syncwarp();
   }
@@ -360,10 +361,11 @@ struct ChunkSmem {
 };
 
 // A CTA takes four consecutive tiles of the heads of one key group, which share K and Q; they may
-// belong to different heads.  Three CTAs (168 registers a thread) fill an SM with three warps on
-// each of its quarters, whatever the headdim.
-template <int N, int MINB>
-__global__ void __launch_bounds__(kWarps * 32, MINB) delta_chunk_kernel(const DeltaChunkParams p) {
+// belong to different heads.  Two CTAs (up to 255 registers a thread) put two warps on each quarter
+// of an SM, whatever the headdim; three CTAs of 168 registers were slower (844 against 819 us for
+// 8 x 2048 tokens of 128 heads of 80).
+template <int N>
+__global__ void __launch_bounds__(kWarps * 32, 2) delta_chunk_kernel(const DeltaChunkParams p) {
   using L = ChunkSmem<N>;
   extern __shared__ __align__(128) unsigned char sm[];
   __shared__ uint64_t full[kStages], empty[kStages];
@@ -465,14 +467,15 @@ __global__ void __launch_bounds__(kWarps * 32, MINB) delta_chunk_kernel(const De
     // P = S K^T and O = S Q^T (state rows x tokens)
     float Pm[kTiles][4] = {}, O[kTiles][4] = {};
     __half2 smax = __float2half2_rn(0.0f);
+    uint32_t sa[2][2][4];     // pieces of 16 columns, of the next 16
+    auto pieces = [&](int ks, int e) {
+      split2(S[2 * ks + (e >> 1)][2 * (e & 1)], S[2 * ks + (e >> 1)][2 * (e & 1) + 1], sa[ks & 1][0][e], sa[ks & 1][1][e]);
+      smax = __hmax2(smax, __habs2(*reinterpret_cast<__half2*>(&sa[ks & 1][0][e])));
+    };
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pieces(0, e);
 #pragma unroll
     for (int ks = 0; ks < N / 16; ++ks) {
-      uint32_t a[2][4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        split2(S[2 * ks + (e >> 1)][2 * (e & 1)], S[2 * ks + (e >> 1)][2 * (e & 1) + 1], a[0][e], a[1][e]);
-        smax = __hmax2(smax, __habs2(*reinterpret_cast<__half2*>(&a[0][e])));
-      }
       uint32_t b[kTiles / 2][4], d[kTiles / 2][4];
 #pragma unroll
       for (int j = 0; j < kTiles; j += 2) {
@@ -480,13 +483,16 @@ __global__ void __launch_bounds__(kWarps * 32, MINB) delta_chunk_kernel(const De
         ldsm4(b[j / 2], st + off);
         ldsm4(d[j / 2], st + kC * N * 2 + off);
       }
-      // products into one accumulator are apart by a round over the tiles
+      // products into one accumulator are apart by a round over the tiles; the next pieces between them
 #pragma unroll
-      for (int j = 0; j < kTiles; ++j) mma16816(Pm[j], a[0], b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
-#pragma unroll
-      for (int j = 0; j < kTiles; ++j) mma16816(O[j], a[0], d[j / 2][2 * (j & 1)], d[j / 2][2 * (j & 1) + 1]);
-#pragma unroll
-      for (int j = 0; j < kTiles; ++j) mma16816(Pm[j], a[1], b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
+      for (int x = 0; x < 3 * kTiles; ++x) {
+        const int j = x % kTiles, r = x / kTiles;
+        if (r == 1)
+          mma16816(O[j], sa[ks & 1][0], d[j / 2][2 * (j & 1)], d[j / 2][2 * (j & 1) + 1]);
+        else
+          mma16816(Pm[j], sa[ks & 1][r / 2], b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
+        if (x % 3 == 0 && ks + 1 < N / 16) pieces(ks + 1, x / 3);
+      }
     }
     // r = beta (v - e^G S k), in place
     float rmax = 0.0f;
