@@ -16,6 +16,10 @@ weights and cache must live on a CUDA device.
 Cold storage: ``cold="fp32"`` reproduces the reference's ``cold_bf16=0`` to fp32 rounding;
 ``"bf16"`` / ``"fp8"`` keep the cold slice only in that dtype (dequantise, replay,
 requantise every c tokens), where the reference re-snapshots a full fp32 state.
+Beam search: the pool's slots follow the beams.  When the cache's rows are reordered
+(``generate(num_beams=...)``, :func:`beam_search`), ``reorder_slots`` gives every row the slot of the
+beam it continues and copies states only where a beam was forked.
+
 ``cold="off"`` is the hot-only self-speculative draft model (the reference's
 ``install(..., cold="off")``, scale/v4_fused_decode.py:140-142 and :49-55): after the prefill
 split, every decode token runs ``draft_state_update`` on a draft copy of the hot slice, with no
@@ -28,9 +32,11 @@ import math
 import torch
 import torch.nn.functional as F
 
+from .beam import beam_select
 from .ops import (conv_step, draft_state_update, gated_rmsnorm, mamba_chunk_scan_combined, prefill_split, rot_flat,
                   tiered_state_update)
 from .pool import TieredSlotPool
+from .slots import StateBuffers, reorder_slots
 
 _MODES = {(0, 0): "stale", (1, 0): "corr", (0, 1): "coldoff"}
 
@@ -184,6 +190,22 @@ def _lean_prefill(self, input_states, cache_params, attention_mask):
     return self.out_proj(scan_output.to(self.out_proj.weight.dtype))
 
 
+def _follow_beams(layer, st) -> None:
+    """Let the pool's slots follow the rows of a cache layer when beam search reorders them."""
+    if getattr(layer, "_nssm", None) is st:
+        return
+    rows_of_cache = layer.reorder_cache
+
+    def reorder_cache(beam_idx):
+        rows_of_cache(beam_idx)
+        slots = st["slots"]
+        if st["draft"] is not None:
+            reorder_slots(StateBuffers([st["draft"]]), slots, beam_idx.to(slots.device))
+        st["slots"] = reorder_slots(st["pool"], slots, beam_idx.to(slots.device))
+
+    layer._nssm, layer.reorder_cache = st, reorder_cache
+
+
 def _dispatch(self, input_states, cache_params=None, attention_mask=None):
     st = self._nssm
     seq_len = input_states.shape[1]
@@ -209,6 +231,7 @@ def _dispatch(self, input_states, cache_params=None, attention_mask=None):
             st["draft"] = pool.new_draft()[0] if st["cold"] == "off" else None
         prefill_split(pool, 0, ssm.contiguous(), st["slots"])
         st["draft_fresh"] = True
+        _follow_beams(cache_params.layers[self.layer_idx], st)
     return out
 
 
@@ -236,3 +259,43 @@ def install(model, pb: int = 32, c: int = 16, cold: str | None = None, corr: int
             m.torch_forward = _dispatch.__get__(m)
             n += 1
     return n
+
+
+@torch.no_grad()
+def beam_search(model, input_ids: torch.Tensor, num_beams: int, max_new_tokens: int, eos_token_id: int | None = None,
+                attention_mask: torch.Tensor | None = None):
+    """Beam search on an installed model: ``input_ids [b, T]`` -> ``(sequences [b, num_beams,
+    T + new], scores [b, num_beams])``, best first, the scores sums of log probabilities.
+
+    Every token is one ``beam_select`` over the beams' logits and one reorder of the cache (and with
+    it of the pools' slots).  A beam that ends with ``eos_token_id`` keeps its score and is filled up
+    with it; the search stops when every beam has ended."""
+    b, T = input_ids.shape
+    K, dev = num_beams, input_ids.device
+    ids = input_ids.repeat_interleave(K, 0)
+    mask = None if attention_mask is None else attention_mask.repeat_interleave(K, 0)
+    seqs = ids.view(b, K, T)
+    scores = torch.full((b, K), float("-inf"), device=dev)   # the first continuations all come from beam 0
+    scores[:, 0] = 0.0
+    finished = None
+    first_row = torch.arange(0, b * K, K, device=dev)[:, None]
+    cache, step = None, ids
+    for i in range(max_new_tokens):
+        out = model(input_ids=step, attention_mask=mask, past_key_values=cache, use_cache=True)
+        cache = out.past_key_values
+        logits = out.logits[:, -1].view(b, K, -1)
+        if logits.dtype not in (torch.bfloat16, torch.float32):
+            logits = logits.float()
+        chosen = beam_select(logits, scores, K, finished, eos_token_id)
+        scores, parents, tokens = chosen[:3]
+        seqs = torch.cat([seqs.gather(1, parents.long()[..., None].expand_as(seqs)), tokens[..., None].to(seqs.dtype)], -1)
+        if eos_token_id is not None:
+            finished = chosen[3]
+            if bool(finished.all()):
+                break
+        if i + 1 < max_new_tokens:
+            cache.reorder_cache((first_row + parents).reshape(-1))
+            step = tokens.reshape(-1, 1).to(input_ids.dtype)
+            if mask is not None:
+                mask = torch.cat([mask, mask.new_ones(b * K, 1)], 1)
+    return seqs, scores
