@@ -53,10 +53,10 @@ int launch_chunks(nssm::DeltaChunkParams& p, void* ws, cudaStream_t st) {
   auto walk = nssm::delta_chunk_kernel<N>;
   p.img = static_cast<unsigned char*>(ws);
   p.blk = p.img + (int64_t)p.chunks * p.s.G * nssm::kImgBytes<N>;
-  const int smem = nssm::ChunkSmem<N>::bytes(p.heads);
+  const int smem = nssm::ChunkSmem<N>::bytes(p.stages, p.heads);
   cudaError_t e = cudaFuncSetAttribute(prep, cudaFuncAttributeMaxDynamicSharedMemorySize, nssm::PrepSmem<N>::kBytes);
   if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(walk, cudaFuncAttributeMaxDynamicSharedMemorySize, nssm::ChunkSmem<N>::bytes(nssm::kWarps));
+    e = cudaFuncSetAttribute(walk, cudaFuncAttributeMaxDynamicSharedMemorySize, nssm::ChunkSmem<N>::bytes(nssm::kChunkStages, nssm::kWarps));
   if (e == cudaSuccess) e = cudaFuncSetAttribute(walk, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -178,6 +178,7 @@ int nssm_delta_scan(const nssm_delta_scan_args* a, void* stream) {
   c.tile_groups = (a->nheads / a->ngroups * c.tiles + nssm::kWarps - 1) / nssm::kWarps;
   // four tiles from a multiple of four on lie in one or two heads of two tiles or more
   c.heads = c.tiles == 1 ? nssm::kWarps : c.tiles % nssm::kWarps ? 2 : 1;
+  c.stages = c.heads == 1 ? 4 : 3;   // as many as two CTAs of an SM have room for
   return a->dstate == 64 ? launch_chunks<64>(c, a->workspace, st) : launch_chunks<128>(c, a->workspace, st);
 }
 

@@ -54,6 +54,7 @@ struct DeltaChunkParams {
   int tiles;             // 16-row tiles of a head
   int tile_groups;       // CTAs per key group and sequence
   int heads;             // heads of a CTA's tiles at most
+  int stages;            // chunks in shared memory
 };
 
 __device__ __forceinline__ uint32_t bf2(float lo, float hi) {
@@ -105,6 +106,19 @@ __device__ __forceinline__ void stsm4t(uint32_t addr, uint32_t a, uint32_t b, ui
                : "memory");
 }
 __device__ __forceinline__ uint32_t sm32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+// A warp's bounded wait: one test that does not suspend (a phase that is over costs a fraction of a
+// suspending try), then the tries; every lane observes the barrier.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t polls) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  if (__all_sync(0xffffffffu, ok)) return true;
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, polls));
+}
+
 // 16 bytes global -> shared, or zeros
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
@@ -348,7 +362,10 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const DeltaChu
 }
 
 // ---------------------------------------------------------------- the walk over the chunks
-constexpr int kStages = 2;    // chunks in shared memory (three or four measured the same)
+// Chunks in shared memory.  Copies are issued (stages - 2) chunks ahead, into a stage that was in use
+// two chunks ago: a chunk's copies take about as long as its work, and the warp that issues them
+// should not wait for the slowest warp's last chunk.
+constexpr int kChunkStages = 4;
 constexpr int kWarps = 4;     // 16-row tiles of a CTA, one on each quarter of an SM
 // A warp's own V tile: 32 tokens of 16 values, at a pitch that puts 8 rows into 8 bank groups; the
 // next chunk's lies beside it.  y leaves through it.
@@ -357,7 +374,9 @@ constexpr int kVBytes = kC * kVPitch;
 template <int N>
 struct ChunkSmem {
   static __host__ __device__ constexpr int stage(int heads) { return (kImgBytes<N> + heads * kBlkBytes + 127) / 128 * 128; }
-  static __host__ __device__ constexpr int bytes(int heads) { return kStages * stage(heads) + kWarps * 2 * kVBytes; }
+  static __host__ __device__ constexpr int bytes(int stages, int heads) {
+    return stages * stage(heads) + kWarps * 2 * kVBytes;
+  }
 };
 
 // A CTA takes four consecutive tiles of the heads of one key group, which share K and Q; they may
@@ -368,7 +387,7 @@ template <int N>
 __global__ void __launch_bounds__(kWarps * 32, 2) delta_chunk_kernel(const DeltaChunkParams p) {
   using L = ChunkSmem<N>;
   extern __shared__ __align__(128) unsigned char sm[];
-  __shared__ uint64_t full[kStages], empty[kStages];
+  __shared__ uint64_t full[kChunkStages], empty[kChunkStages];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int grp = blockIdx.x / p.tile_groups, tg = blockIdx.x - grp * p.tile_groups, s = blockIdx.y;
   int batch, t0, len;
@@ -383,7 +402,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) delta_chunk_kernel(const Delta
   const int hr = (tg * kWarps + warp) / p.tiles;                // the warp's
   const int h = grp * rep + hr, row_h = ((tg * kWarps + warp) - hr * p.tiles) * 16;
   if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < kChunkStages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], warps);
     }
@@ -394,17 +413,16 @@ __global__ void __launch_bounds__(kWarps * 32, 2) delta_chunk_kernel(const Delta
   const int nchunk = (len + kC - 1) / kC;
   const int slot0 = chunk_base(p, s);
   const uint32_t base = sm32(sm);
-  const int stage = L::stage(p.heads);
+  const int stage = L::stage(p.heads), stages = p.stages, ahead = p.stages - 2;
   const __nv_bfloat16* gv = p.s.v + batch * p.s.v_b + (int64_t)t0 * p.s.v_t + h * p.s.P + row_h;
   const unsigned char* gimg = p.img + ((int64_t)slot0 * p.s.G + grp) * kImgBytes<N>;
   const unsigned char* gblk = p.blk + ((int64_t)slot0 * p.s.H + grp * rep + h0) * kBlkBytes;
 
-  // K, Q, T and M of chunk c into its stage (warp 0); the stage was read before, by ordinary loads
+  // K, Q, T and M of chunk c into its stage, by one warp
   auto load = [&](int c) {
-    unsigned char* st = sm + (c % kStages) * stage;
-    uint64_t* bar = &full[c % kStages];
+    unsigned char* st = sm + (c % stages) * stage;
+    uint64_t* bar = &full[c % stages];
     if (lane == 0) {
-      fence_proxy_async_smem();
       mbar_expect_tx(bar, kImgBytes<N> + nh * kBlkBytes);
       bulk_g2s(st, gimg + (int64_t)c * p.s.G * kImgBytes<N>, kImgBytes<N>, bar);
       bulk_g2s(st + kImgBytes<N>, gblk + (int64_t)c * p.s.H * kBlkBytes, nh * kBlkBytes, bar);
@@ -412,7 +430,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) delta_chunk_kernel(const Delta
     __syncwarp();
   };
   // the warp's V tile of chunk c, zeros for tokens that are not there
-  const uint32_t vbase = base + kStages * stage + warp * 2 * kVBytes;
+  const uint32_t vbase = base + stages * stage + warp * 2 * kVBytes;
   auto load_v = [&](int c) {
     const int nt = len - c * kC;
 #pragma unroll
@@ -444,22 +462,33 @@ __global__ void __launch_bounds__(kWarps * 32, 2) delta_chunk_kernel(const Delta
 #pragma unroll
     for (int e = 0; e < 4; ++e) S[t][e] *= su.s;
   bool ok = true;
-  int loaded = 0;       // chunks whose copies warp 0 has issued
-  if (warp == 0 && nchunk > 0) load(loaded++);
+  if (warp == 0)
+    for (int c = 0; c < min(ahead, nchunk); ++c) load(c);
   if (nchunk > 0) load_v(0);
   cp_commit();
+  int turn = 0;         // the warp that issues the next copies
+  int si = 0, phase = 0;                // the chunk's stage
+  int last = min(ahead, nchunk) - 1;   // the last chunk whose copies this warp may have issued
   for (int c = 0; c < nchunk && ok; ++c) {
-    const int si = c % kStages;
-    if (warp == 0 && loaded < nchunk) {
+    const int next = c + ahead;
+    if (warp == turn && next < nchunk) {
       // the stage is free once every warp is through the chunk that was in it
-      if (loaded >= kStages)
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[loaded % kStages], (loaded / kStages - 1) & 1, p.s.polls));
-      if (ok) load(loaded++);
+      if (next >= stages)
+        ok = warp_wait(&empty[next % stages], (next / stages - 1) & 1, p.s.polls);
+      if (ok) {
+        load(next);
+        last = next;
+      }
+    }
+    turn = turn + 1 == warps ? 0 : turn + 1;
+    if (c && ++si == stages) {
+      si = 0;
+      phase ^= 1;
     }
     if (c + 1 < nchunk) load_v(c + 1);
     cp_commit();
     cp_wait<1>();
-    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[si], (c / kStages) & 1, p.s.polls)) && ok;
+    ok = warp_wait(&full[si], phase, p.s.polls) && ok;
     if (!ok) break;
     const uint32_t st = base + si * stage, vt = vbase + (c & 1) * kVBytes;
     const unsigned char* blk = sm + si * stage + kImgBytes<N> + (hr - h0) * kBlkBytes;
@@ -618,10 +647,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) delta_chunk_kernel(const Delta
     if (lane == 0) mbar_arrive(&empty[si]);
   }
   if (!ok) {
-    // a wait ran out: the copies still in flight land (bounded) before the shared memory goes
+    // a wait ran out: this warp's copies still in flight land (bounded) before it leaves
     if (lane == 0 && p.s.status) atomicOr(p.s.status, STATUS_TIMEOUT);
-    if (warp == 0)
-      for (int c = max(0, loaded - kStages); c < loaded; ++c) mbar_wait_bounded(&full[c % kStages], (c / kStages) & 1, p.s.polls);
+    cp_wait<0>();
+    for (int c = max(0, last - ahead); c <= last; ++c)
+      if ((c < ahead ? 0 : (c - ahead) % warps) == warp) mbar_wait_bounded(&full[c % stages], (c / stages) & 1, p.s.polls);
     return;
   }
   if (p.s.fin)
