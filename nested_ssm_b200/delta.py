@@ -100,16 +100,17 @@ def gated_delta_state_update(state: torch.Tensor, q, k, v, g, beta, scale: float
     return out
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``[b, T, heads, dim]`` with packed (heads, dim), 16-byte aligned tokens and no broadcast
-    axis: what the kernel loads; copied when it is not so."""
-    b, T, h, d = t.shape
-    s = t.stride()
-    if s[3] != 1 or s[2] != d or s[1] % 8 or s[0] % 8 or t.data_ptr() % 16:
+def _rows(t: torch.Tensor):
+    """(t, stride_b, stride_t) of ``[b, T, heads, dim]`` with packed (heads, dim), 16-byte aligned
+    tokens and no broadcast axis: what the kernel loads; copied when it is not so."""
+    d = t.shape[3]
+    s0, s1, s2, s3 = t.stride()
+    if s3 != 1 or s2 != d or s1 % 8 or s0 % 8 or t.data_ptr() % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:     # a contiguous view that begins inside a 16-byte piece
             t = t.clone()
-    return t
+        s0, s1, _, _ = t.stride()
+    return t, s0, s1
 
 
 def gated_delta_chunk_scan(q, k, v, g, beta, scale: float | None = None, initial_states=None, cu_seqlens=None,
@@ -126,36 +127,41 @@ def gated_delta_chunk_scan(q, k, v, g, beta, scale: float | None = None, initial
     do not ascend inside ``[0, T]`` are skipped and set bit 3 of the int32 ``status``.  Otherwise
     n == b.  ``initial_states [n, H, P, N]`` fp32 (zeros without them); ``final_states`` may be the
     same tensor.  ``g`` may be ``-inf`` (the state is forgotten)."""
-    if q.dim() != 4 or k.shape != q.shape or v.dim() != 4 or g.dim() != 3 or beta.dim() != 3:
+    qs, vs = q.shape, v.shape
+    if len(qs) != 4 or k.shape != qs or len(vs) != 4:
         raise ValueError("q / k [b, T, G, N], v [b, T, H, P], g / beta [b, T, H] expected")
-    b, T, G, N = q.shape
-    H, P = v.shape[2:]
-    if v.shape[:2] != (b, T) or g.shape != (b, T, H) or beta.shape != (b, T, H):
-        raise ValueError(f"shape mismatch: q {tuple(q.shape)} v {tuple(v.shape)} g {tuple(g.shape)} "
-                         f"beta {tuple(beta.shape)}")
+    b, T, G, N = qs
+    _, _, H, P = vs
+    if vs[:2] != (b, T) or g.shape != (b, T, H) or beta.shape != (b, T, H):
+        raise ValueError(f"shape mismatch: q {tuple(qs)} v {tuple(vs)} g {tuple(g.shape)} beta {tuple(beta.shape)}")
     if q.dtype != torch.bfloat16 or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
         raise ValueError("q, k and v must be bf16")
     _no_grad(q, k, v, g, beta, initial_states)
-    n = b
+    n, cu = b, 0
     if cu_seqlens is not None:
-        if b != 1 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+        if b != 1 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
             raise ValueError("cu_seqlens [n + 1] needs packed inputs with b == 1")
-        n = cu_seqlens.numel() - 1
+        n = cu_seqlens.shape[0] - 1
         cu_seqlens = _indices(cu_seqlens, n + 1, "cu_seqlens")
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    if g.stride(2) != 1:
-        g = g.contiguous()
-    if beta.stride(2) != 1:
-        beta = beta.contiguous()
+        cu = cu_seqlens.data_ptr()
+    (q, q0, q1), (k, k0, k1), (v, v0, v1) = _rows(q), _rows(k), _rows(v)
+    g0, g1, g2 = g.stride()
+    b0, b1, b2 = beta.stride()
+    if g2 != 1 or b2 != 1:
+        g, beta = g.contiguous(), beta.contiguous()
+        (g0, g1, _), (b0, b1, _) = g.stride(), beta.stride()
     inner = (P * N, N, 1)
+    init = init0 = fin = fin0 = 0
     if initial_states is not None:
         if initial_states.shape != (n, H, P, N):
             raise ValueError(f"initial_states must be [{n}, {H}, {P}, {N}], got {tuple(initial_states.shape)}")
         if (initial_states.dtype != torch.float32 or initial_states.stride()[1:] != inner
                 or initial_states.stride(0) % 4 or initial_states.data_ptr() % 16):
             initial_states = initial_states.float().contiguous()
+        init, init0 = initial_states.data_ptr(), initial_states.stride(0)
+    where = q.device
     if out is None:
-        out = torch.empty(b, T, H, P, dtype=torch.bfloat16, device=q.device)
+        out = torch.empty(b, T, H, P, dtype=torch.bfloat16, device=where)
     elif out.shape != (b, T, H, P) or out.dtype != torch.bfloat16 or out.stride()[2:] != (P, 1):
         raise ValueError("out must be bf16 [b, T, H, P] with packed (H, P)")
     if final_states is not None:
@@ -163,19 +169,20 @@ def gated_delta_chunk_scan(q, k, v, g, beta, scale: float | None = None, initial
                 or final_states.stride()[1:] != inner):
             raise ValueError(f"final_states must be fp32 [{n}, {H}, {P}, {N}] with contiguous rows")
     elif return_final_states:
-        final_states = torch.empty(n, H, P, N, dtype=torch.float32, device=q.device)
+        final_states = torch.empty(n, H, P, N, dtype=torch.float32, device=where)
+    if final_states is not None:
+        fin, fin0 = final_states.data_ptr(), final_states.stride(0)
     if status is not None:
         _check_status(status)
     dev = _lib.device_index(q, k, v, g, beta, cu_seqlens, initial_states, out, final_states, status)
     lib = _lib.load()
-    nbytes = lib.nssm_delta_scan_workspace_bytes(n, T, H, G, N, int(cu_seqlens is not None))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    nbytes = lib.nssm_delta_scan_workspace_bytes(n, T, H, G, N, 1 if cu else 0)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=where) if nbytes else None
+    o0, o1, _, _ = out.stride()
     a = _pack_scan(
         n, T, H, G, P, N, nssm_dtype(g.dtype), nssm_dtype(beta.dtype), N ** -0.5 if scale is None else float(scale), 0,
-        q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2], g.data_ptr(),
-        *g.stride()[:2], beta.data_ptr(), *beta.stride()[:2], ptr(cu_seqlens),
-        ptr(initial_states), 0 if initial_states is None else initial_states.stride(0), out.data_ptr(), *out.stride()[:2],
-        ptr(final_states), 0 if final_states is None else final_states.stride(0), ptr(ws), nbytes, ptr(status))
+        q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, g.data_ptr(), g0, g1, beta.data_ptr(), b0, b1,
+        cu, init, init0, out.data_ptr(), o0, o1, fin, fin0, 0 if ws is None else ws.data_ptr(), nbytes,
+        0 if status is None else status.data_ptr())
     _lib.call(lib.nssm_delta_scan, dev, a)
     return (out, final_states) if return_final_states else out
