@@ -150,6 +150,7 @@ int nssm_delta_scan(const nssm_delta_scan_args* a, void* stream) {
   const int64_t row = (int64_t)a->nheads * a->headdim * a->dstate;
   if (a->final_states && a->batch > 1 && a->final_stride_b < row)
     return fail(NSSM_ERR_INVALID, "final_stride_b smaller than a state");
+  if (ws_chunks(a->batch, a->seqlen, a->cu_seqlens != nullptr) > (1 << 30)) return fail(NSSM_ERR_INVALID, "batch * seqlen too large");
   nssm::DeltaScanParams p{};
   p.B = a->batch; p.T = a->seqlen; p.H = a->nheads; p.G = a->ngroups; p.P = a->headdim;
   p.g_bf16 = a->g_dtype == NSSM_BF16; p.beta_bf16 = a->beta_dtype == NSSM_BF16;

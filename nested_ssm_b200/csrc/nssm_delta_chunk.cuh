@@ -456,7 +456,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) delta_chunk_kernel(const Delta
   float m0 = 0.0f;
 #pragma unroll
   for (int t = 0; t < N / 8; ++t) m0 = amax4(S[t], m0);
-  Pow2 su = warp_scale(m0);   // the registers hold su.s S, no element of it above 2^15
+  Pow2 su{1.0f, 1.0f};        // the registers hold su.s S, no element of it above 2^15
+  if (nchunk > 0) su = warp_scale(m0);
 #pragma unroll
   for (int t = 0; t < N / 8; ++t)
 #pragma unroll

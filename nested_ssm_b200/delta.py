@@ -61,8 +61,9 @@ def gated_delta_state_update(state: torch.Tensor, q, k, v, g, beta, scale: float
         raise ValueError(f"state must be an fp32 [S, H, P, N] tensor, got {tuple(state.shape)} {state.dtype}")
     S, H, P, N = state.shape
     ss = state.stride()
-    if ss[1:] != (P * N, N, 1):
+    if ss[1:] != (P * N, N, 1) and not state[:1].flatten(0, 1).is_contiguous():   # (axes of one have any stride)
         raise ValueError("the heads of a slot must be contiguous in state")
+    s0 = ss[0] if S > 1 else H * P * N
     qs = q.shape
     if len(qs) != 3 or k.shape != qs or qs[2] != N:
         raise ValueError(f"q and k must be [b, G, {N}], got {tuple(q.shape)} and {tuple(k.shape)}")
@@ -93,7 +94,7 @@ def gated_delta_state_update(state: torch.Tensor, q, k, v, g, beta, scale: float
     b0, b1 = beta.stride()
     a = _pack_step(
         b, S, H, G, P, N, nssm_dtype(dt), nssm_dtype(g.dtype), nssm_dtype(beta.dtype), nssm_dtype(out.dtype),
-        int(pad_slot_id), N ** -0.5 if scale is None else float(scale), state.data_ptr(), ss[0], q.data_ptr(), q0, q1,
+        int(pad_slot_id), N ** -0.5 if scale is None else float(scale), state.data_ptr(), s0, q.data_ptr(), q0, q1,
         k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, g.data_ptr(), g0, g1, beta.data_ptr(), b0, b1,
         0 if idx is None else idx.data_ptr(), out.data_ptr(), o0, o1, 0 if status is None else status.data_ptr())
     _lib.call(_lib.load().nssm_delta_step, dev, a)
@@ -126,7 +127,8 @@ def gated_delta_chunk_scan(q, k, v, g, beta, scale: float | None = None, initial
     the rows of ``out`` outside every sequence are left as they were.  Sequences whose bounds
     do not ascend inside ``[0, T]`` are skipped and set bit 3 of the int32 ``status``.  Otherwise
     n == b.  ``initial_states [n, H, P, N]`` fp32 (zeros without them); ``final_states`` may be the
-    same tensor.  ``g`` may be ``-inf`` (the state is forgotten)."""
+    same tensor.  ``g`` may be ``-inf`` (the state is forgotten); any other value of a sequence that
+    is not finite reaches every output of its 32-token block, those before it too, and the state."""
     qs, vs = q.shape, v.shape
     if len(qs) != 4 or k.shape != qs or len(vs) != 4:
         raise ValueError("q / k [b, T, G, N], v [b, T, H, P], g / beta [b, T, H] expected")
@@ -150,23 +152,25 @@ def gated_delta_chunk_scan(q, k, v, g, beta, scale: float | None = None, initial
     if g2 != 1 or b2 != 1:
         g, beta = g.contiguous(), beta.contiguous()
         (g0, g1, _), (b0, b1, _) = g.stride(), beta.stride()
-    inner = (P * N, N, 1)
+    def packed(t):     # the heads of a sequence are contiguous (axes of one have any stride)
+        return t.stride()[1:] == (P * N, N, 1) or t[:1].flatten(0, 1).is_contiguous()
+
     init = init0 = fin = fin0 = 0
     if initial_states is not None:
         if initial_states.shape != (n, H, P, N):
             raise ValueError(f"initial_states must be [{n}, {H}, {P}, {N}], got {tuple(initial_states.shape)}")
-        if (initial_states.dtype != torch.float32 or initial_states.stride()[1:] != inner
-                or initial_states.stride(0) % 4 or initial_states.data_ptr() % 16):
+        if (initial_states.dtype != torch.float32 or not packed(initial_states) or initial_states.stride(0) % 4
+                or initial_states.data_ptr() % 16):
             initial_states = initial_states.float().contiguous()
         init, init0 = initial_states.data_ptr(), initial_states.stride(0)
     where = q.device
     if out is None:
         out = torch.empty(b, T, H, P, dtype=torch.bfloat16, device=where)
-    elif out.shape != (b, T, H, P) or out.dtype != torch.bfloat16 or out.stride()[2:] != (P, 1):
+    elif out.shape != (b, T, H, P) or out.dtype != torch.bfloat16 or (
+            out.stride()[2:] != (P, 1) and not out[:1, :1].flatten(0, 2).is_contiguous()):
         raise ValueError("out must be bf16 [b, T, H, P] with packed (H, P)")
     if final_states is not None:
-        if (final_states.shape != (n, H, P, N) or final_states.dtype != torch.float32
-                or final_states.stride()[1:] != inner):
+        if final_states.shape != (n, H, P, N) or final_states.dtype != torch.float32 or not packed(final_states):
             raise ValueError(f"final_states must be fp32 [{n}, {H}, {P}, {N}] with contiguous rows")
     elif return_final_states:
         final_states = torch.empty(n, H, P, N, dtype=torch.float32, device=where)

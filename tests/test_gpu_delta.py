@@ -413,3 +413,55 @@ def test_on_another_stream_and_in_a_replayed_graph():
         g.replay()
     for o in outs:
         assert torch.equal(o[0], y) and torch.equal(o[1], S) and torch.equal(o[2], z)
+
+
+def test_axes_of_one_may_have_any_stride():
+    """One head, one sequence: the strides of such axes say nothing."""
+    from nested_ssm_b200 import gated_delta_chunk_scan, gated_delta_state_update
+    P, N, T = 32, 64, 40
+    d = _inputs(1, T, 1, 1, P, N, seed=21)
+    yr, Sr = OD.gated_delta_scan(d["q"], d["k"], d["v"], d["g"], d["beta"], S0=d["s0"])
+    odd = lambda t, *s: torch.as_strided(t, t.shape, s)  # noqa: E731
+    out = odd(torch.zeros(1, T, 1, P, device="cuda", dtype=torch.bfloat16), 8, P, 5, 1)
+    fin = odd(torch.zeros(1, 1, P, N, device="cuda"), 4, 12, N, 1)
+    y, S = gated_delta_chunk_scan(odd(d["q"], 8, N, 3, 1), d["k"], d["v"], d["g"], d["beta"],
+                                  initial_states=odd(d["s0"], 8, 4, N, 1), return_final_states=True, out=out,
+                                  final_states=fin)
+    _check_y(y, yr)
+    _check_state(S, Sr)
+    state = odd(d["s0"].clone(), 0, 7, N, 1)
+    x = [d[n][:, 0] for n in ("q", "k", "v", "g", "beta")]
+    z = gated_delta_state_update(state, *x)
+    _check_y(z, yr[:, 0])
+
+
+def test_wide_ranges_of_values():
+    """Keys of very different lengths from token to token (beta holds their step in range), values up to
+    1e4 and down to 1e-4, a state of rows that differ by 1e4: the scales of the split operands."""
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    b, T, H, G, P, N = 1, 150, 2, 1, 32, 128
+    d = _inputs(b, T, H, G, P, N, seed=22)
+    g = torch.Generator(device="cuda").manual_seed(23)
+    length = 10.0 ** (2 * torch.rand(b, T, 1, 1, generator=g, device="cuda") - 1)
+    d["k"] = (d["k"].float() * length).bfloat16()
+    d["beta"] = d["beta"] / d["k"].float().square().sum(-1).expand(b, T, H)
+    d["q"] = (d["q"].float() * 10.0 ** (6 * torch.rand(b, T, 1, 1, generator=g, device="cuda") - 3)).bfloat16()
+    d["v"] = (d["v"].float() * 10.0 ** (8 * torch.rand(b, T, 1, 1, generator=g, device="cuda") - 4)).bfloat16()
+    d["s0"] *= 10.0 ** (4 * torch.rand(b, H, P, 1, generator=g, device="cuda"))
+    y, S = gated_delta_chunk_scan(d["q"], d["k"], d["v"], d["g"], d["beta"], initial_states=d["s0"], return_final_states=True)
+    yr, Sr = OD.gated_delta_scan(d["q"], d["k"], d["v"], d["g"], d["beta"], S0=d["s0"])
+    _check_state(S, Sr)
+    assert _rel(y, yr) <= Y_TOL
+
+
+def test_a_value_that_is_not_finite_stays_in_its_sequence_and_block():
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    d = _inputs(2, 130, 2, 1, 32, 64, seed=24)
+    yr, Sr = OD.gated_delta_scan(d["q"], d["k"], d["v"], d["g"], d["beta"])
+    d["v"][0, 70, 1, 3] = float("nan")
+    y, S = gated_delta_chunk_scan(d["q"], d["k"], d["v"], d["g"], d["beta"], return_final_states=True)
+    _check_y(y[1], yr[1])
+    _check_state(S[1], Sr[1])
+    _check_y(y[0, :64], yr[0, :64])                      # blocks of 32 tokens before it
+    assert bool(torch.isnan(y[0, 70:, 1, 3]).all())
+    _check_y(y[0, :, 0], yr[0, :, 0])                    # the other head

@@ -191,3 +191,12 @@ def test_slot_entries(buf, args):
         _err(lib.nssm_slot_copy(b, d["nbuf"], d["S"], p, p, d["rows"], -1, p, d["ws"], None, None))
         _err(lib.nssm_slot_compact(b, d["nbuf"], d["S"], p, d["rows"], -1, p, p, d["ws"], None, None))
     assert lib.nssm_slot_workspace_bytes(8) == 72 and lib.nssm_slot_workspace_bytes(0) == 0
+
+
+def test_delta_scan_refuses_too_many_blocks():
+    a = _fill(_lib.NssmDeltaScanArgs(), **{**DELTA, "batch": 65535, "seqlen": 1 << 20, "q_stride_t": 128, "k_stride_t": 128,
+                                           "v_stride_t": 128, "y_stride_t": 128, "q_stride_b": 128, "k_stride_b": 128,
+                                           "v_stride_b": 128, "y_stride_b": 128, "final_stride_b": 8192, "init_stride_b": 8192,
+                                           "workspace_bytes": 1 << 62, "cu_seqlens": None})
+    _err(_lib.load().nssm_delta_scan(C.byref(a), None))
+    assert "too large" in _lib.load().nssm_last_error().decode()
