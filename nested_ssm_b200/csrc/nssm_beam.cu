@@ -70,6 +70,25 @@ __device__ __forceinline__ uint64_t nth_of_block(uint64_t mine, int n, uint64_t*
   return *result;
 }
 
+// A lower bound of the nth largest of the CTA's values: the nth largest of a few of each warp's.  0
+// where there are too few.
+__device__ __forceinline__ uint32_t lower_bound_of_block(uint32_t mine, int n, uint64_t* sh, uint64_t* result) {
+  const int t = min(32, (2 * n + kBeamWarps - 1) / kBeamWarps), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int k = 0; k < t; ++k) {
+    const uint32_t top = __reduce_max_sync(0xffffffffu, mine);
+    if (lane == 0) sh[warp * t + k] = top;
+    const int who = __ffs(__ballot_sync(0xffffffffu, mine == top)) - 1;
+    if (lane == who) mine = 0;
+  }
+  __syncthreads();
+  const uint64_t v = tid < kBeamWarps * t ? sh[tid] : 0;
+  int rank = 0;
+  for (int i = 0; i < kBeamWarps * t; ++i) rank += sh[i] > v || (sh[i] == v && i < tid);
+  if (tid < kBeamWarps * t && rank == n - 1) *result = v;
+  __syncthreads();
+  return (uint32_t)*result;
+}
+
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
@@ -252,21 +271,8 @@ __global__ void __launch_bounds__(kBeamThreads, BF16 ? 3 : 4) beam_scan_kernel(c
       sum += (s2[0].x + s2[0].y) + (s2[1].x + s2[1].y);
     }
     if (st == step0) {
-      const int t = min(32, (2 * p.n + kBeamWarps - 1) / kBeamWarps);   // maxima of each warp
-      uint32_t mine = order32(mx);
-      for (int k = 0; k < t; ++k) {
-        const uint32_t top = __reduce_max_sync(0xffffffffu, mine);
-        if (lane == 0) sh[warp * t + k] = top;
-        const int who = __ffs(__ballot_sync(0xffffffffu, mine == top)) - 1;
-        if (lane == who) mine = 0;
-      }
-      __syncthreads();
-      const uint64_t v = tid < kBeamWarps * t ? sh[tid] : 0;
-      int rank = 0;
-      for (int i = 0; i < kBeamWarps * t; ++i) rank += sh[i] > v || (sh[i] == v && i < tid);
-      if (tid < kBeamWarps * t && rank == p.n - 1) nth = v;
-      __syncthreads();
-      tau = unorder32((uint32_t)nth);
+      const uint32_t bound = lower_bound_of_block(order32(mx), p.n, sh, &nth);
+      tau = unorder32(bound);
       if (!(tau >= kNegInf)) tau = kNegInf;     // fewer values than that
     }
 #pragma unroll
@@ -403,10 +409,10 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamPara
       best = key[u].hi > best ? key[u].hi : best;
     }
     if (tid == 0) count = 0;
-    // at first the nout-th largest of the threads' best totals: a lower bound
+    // at first a lower bound from the upper halves of the threads' best totals
     BeamKey tau{0, 0};
     if (c0 == 0)
-      tau.hi = nth_of_block(best, p.n, sh, &nth);
+      tau.hi = (uint64_t)lower_bound_of_block((uint32_t)(best >> 32), p.n, sh, &nth) << 32;
     else if (have == p.n)
       tau = cur[p.n - 1];
     __syncthreads();
