@@ -12,16 +12,19 @@
 // A warp owns 16 rows of S for the whole sequence, in the accumulator layout of m16n8k16, which is
 // also that instruction's A layout: every product is taken in its transposed form (S K^T, R^T T^T,
 // S Q^T, U^T M^T, U'^T K), so S, r and u go from one product to the next inside a warp's
-// registers, and warps share only the K, Q, V, T and M tiles.
-#pragma once
-
-#include <cuda_fp16.h>
-
-#include "nssm_delta.cuh"
-#include "nssm_persistent.cuh"
-
-namespace nssm {
-
+// registers, and warps share only the K, Q, T and M tiles.  The chain of a chunk never leaves the
+// register file; on tcgen05 each of its four dependent products would cross tensor memory twice,
+// with the same conversions between, for a 128-row tile that most headdims do not fill.
+//
+// What bounds it: of 2 x 8192 tokens of 32 heads of 128 (531 us; input and output alone 63 us) the walk
+// takes 434 us, one warp on each quarter of 128 SMs, 3030 cycles a chunk, 1470 of them mma (184
+// products of 8 cycles a quarter).  Of 8 x 2048 tokens of 128 heads of 80 (942 us) it takes 757 us,
+// two warps a quarter, the tensor pipe 55 to 73 % busy.  Not kept: chunks of 64 (T costs four times
+// as much a chunk: 1703 against 937 us), bf16 operands in three pieces (316 products a chunk against
+// 184; two pieces leave 3.6e-6 in the state), splitting the columns of S over two or four warps (the
+// part of a chunk that is not split and the exchange take more than is won: 489 -> 619 us), V by one
+// small bulk copy a row (they cost the walk more than its arithmetic).
+//
 // Precision.  The state is fp32, and its products are to be as good: an fp32 operand goes in as two
 // fp16 values (11 bits each, the second holds what the first leaves), scaled by a power of two
 // that keeps the warp's values below 2^15; what is left out is below 2^-22 of a value or 2^-25.  K and Q (bf16) become fp16 exactly, each token scaled by its own power of two
@@ -151,6 +154,8 @@ __device__ __forceinline__ int chunk_base(const DeltaChunkParams& p, int s) {
 }
 
 // ---------------------------------------------------------------- T and M of every chunk
+// 185 us of 942 for 8 x 2048 tokens of 128 heads, 97 of 531 for 2 x 8192 of 32: 0.41 GB and 0.35 GB
+// moved, issue 57 % busy.
 // CTA: one chunk and key group, 4 warps.  k.k and q.k come from the tensor cores once per group
 // (products of bf16 values, fp32 sums); then a warp takes a head at a time, a lane a token row:
 // row i of T solves T (I + A) = I from column i down in fp32 (a backward substitution over A's
