@@ -26,11 +26,21 @@
 // small bulk copy a row (they cost the walk more than its arithmetic).
 //
 // Precision.  The state is fp32, and its products are to be as good: an fp32 operand goes in as two
-// fp16 values (11 bits each, the second holds what the first leaves), scaled by a power of two
-// that keeps the warp's values below 2^15; what is left out is below 2^-22 of a value or 2^-25.  K and Q (bf16) become fp16 exactly, each token scaled by its own power of two
-// (elements below 2^-25 of the token's largest lose bits).  T goes in as two pieces, so only
-// products of two second pieces are left out, 2^-22 of a product.  y is rounded to bf16 (2^-9):
-// the operands of its own products are single fp16 values (2^-12).
+// fp16 values (11 bits each, the second holds what the first leaves), scaled by a power of two that
+// keeps the warp's values below 2^15; what is left out is below 2^-22 of a value or 2^-25.  K and Q
+// (bf16) become fp16 exactly, each token scaled by its own power of two (elements below 2^-25 of the
+// token's largest lose bits).  T goes in as two pieces, so only products of two second pieces are
+// left out, 2^-22 of a product.  y is rounded to bf16 (2^-9): the operands of its own products are
+// single fp16 values (2^-12).
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "nssm_delta.cuh"
+#include "nssm_persistent.cuh"
+
+namespace nssm {
+
 constexpr int kC = 32;          // tokens of a chunk: a warp's lanes are its rows
 constexpr int kTiles = kC / 8;
 constexpr int kSteps = kC / 16;
