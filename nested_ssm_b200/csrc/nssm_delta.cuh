@@ -63,11 +63,13 @@ __device__ __forceinline__ float sum4(float v) {
 // pieces of it in flight at once (128 bytes a thread at N = 128, which is what keeps HBM busy).  k and
 // q of the head wait in shared memory.  The output is read off the old state,
 // y = scale (e^g S q + u (k.q)), so that S k and S q reduce together.  448 rows of 128 heads of 80
-// (4.7 GB): 838 us, 5.6 TB/s; with 8 lanes a row, half the bytes in flight and k and q in registers
-// 1883 us.  Rows are compared with the earlier rows' slots while the state is on its way.
-constexpr int kStepThreads = 320;
+// (4.7 GB): 765 us, 6.2 TB/s with four CTAs of 40 rows an SM (one loads while another computes);
+// 838 us with two of 80, 827 with five at 80 registers; 1883 with 8 lanes a row, half the bytes in
+// flight and k and q in registers.  Rows are compared with the earlier rows' slots while the state is
+// on its way.
+constexpr int kStepRows = 40, kStepThreads = 4 * kStepRows;
 template <int N>
-__global__ void __launch_bounds__(kStepThreads, N == 64 ? 3 : 2) delta_step_kernel(const DeltaStepParams p) {
+__global__ void __launch_bounds__(kStepThreads, 4) delta_step_kernel(const DeltaStepParams p) {
   constexpr int V = N / 16;
   __shared__ float4 sk[N / 4], sq[N / 4];
   const int b = blockIdx.y, h = blockIdx.x / p.ns, slice = blockIdx.x - h * p.ns;
