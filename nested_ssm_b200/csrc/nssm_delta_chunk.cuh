@@ -164,8 +164,9 @@ __device__ __forceinline__ int chunk_base(const DeltaChunkParams& p, int s) {
 }
 
 // ---------------------------------------------------------------- T and M of every chunk
-// 185 us of 942 for 8 x 2048 tokens of 128 heads, 97 of 531 for 2 x 8192 of 32: 0.41 GB and 0.35 GB
-// moved, issue 57 % busy.
+// Bound by latency (a CTA loads, converts, multiplies, then solves) and by issue: 170 us for 8 x 2048
+// tokens of 128 heads, 104 for 2 x 8192 of 32 heads, which move 0.41 and 0.35 GB.  Seven CTAs an SM;
+// with five 174 and 116, with four 178 and 128.
 // CTA: one chunk and key group, 4 warps.  k.k and q.k come from the tensor cores once per group
 // (products of bf16 values, fp32 sums); then a warp takes a head at a time, a lane a token row:
 // row i of T solves T (I + A) = I from column i down in fp32 (a backward substitution over A's
@@ -175,16 +176,17 @@ constexpr int kPitch = kC + 4;    // floats: 16-byte reads of 8 lanes' rows fall
 
 template <int N>
 struct PrepSmem {
-  static constexpr int off_kk = kImgBytes<N>;
+  // the columns of A (4 KB of each warp) take the place of the images once k.k and q.k are there
+  static constexpr int kA = kPrepWarps * kC * kC * 4;
+  static constexpr int off_kk = kImgBytes<N> > kA ? kImgBytes<N> : kA;
   static constexpr int off_qk = off_kk + kC * kPitch * 4;
-  static constexpr int off_a = off_qk + kC * kPitch * 4;        // columns of A, per warp
-  static constexpr int off_g = off_a + kPrepWarps * kC * kC * 4;   // G as two floats, per warp
+  static constexpr int off_g = off_qk + kC * kPitch * 4;        // G as two floats, per warp
   static constexpr int off_s = off_g + kPrepWarps * 2 * kC * 4;    // sk, sq
   static constexpr int kBytes = off_s + 2 * kC * 4;
 };
 
 template <int N>
-__global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const DeltaChunkParams p) {
+__global__ void __launch_bounds__(kPrepThreads, 7) delta_prep_kernel(const DeltaChunkParams p) {
   using L = PrepSmem<N>;
   extern __shared__ __align__(128) unsigned char sm[];
   __shared__ int s_seq;
@@ -272,22 +274,28 @@ __global__ void __launch_bounds__(kPrepThreads) delta_prep_kernel(const DeltaChu
   }
   __syncthreads();
 
-  float* A = reinterpret_cast<float*>(sm + L::off_a) + warp * kC * kC;    // [column][row]
+  float* A = reinterpret_cast<float*>(sm) + warp * kC * kC;    // [column][row]
   float* gh = reinterpret_cast<float*>(sm + L::off_g) + warp * 2 * kC;
   float* gl = gh + kC;
   const int rep = p.s.H / p.s.G;
+  // g and beta of this lane's token, a head ahead
+  const int64_t og = batch * p.s.g_b + (tok + lane) * p.s.g_t, ob = batch * p.s.beta_b + (tok + lane) * p.s.beta_t;
+  float ng = 0.0f, nbeta = 0.0f;
+  auto fetch = [&](int hr) {
+    if (lane < nt && hr < rep) {
+      ng = dl_ld(p.s.g, og + grp * rep + hr, p.s.g_bf16);
+      nbeta = dl_ld(p.s.beta, ob + grp * rep + hr, p.s.beta_bf16);
+    }
+  };
+  fetch(warp);
   for (int hr = warp; hr < rep; hr += kPrepWarps) {
     const int h = grp * rep + hr;
     // G in units of ln 2: a 64-bit prefix sum, so that differences of far sums keep their
     // precision.  Below e^-104 a decay is zero in fp32: the clamp changes none and keeps -inf
     // out of the sums.
-    double G = 0.0;
-    float beta = 0.0f;
-    if (lane < nt) {
-      const float g = dl_ld(p.s.g, batch * p.s.g_b + (tok + lane) * p.s.g_t + h, p.s.g_bf16);
-      G = (g < -120.0f ? -120.0 : (double)g) * 1.4426950408889634;
-      beta = dl_ld(p.s.beta, batch * p.s.beta_b + (tok + lane) * p.s.beta_t + h, p.s.beta_bf16);
-    }
+    double G = (ng < -120.0f ? -120.0 : (double)ng) * 1.4426950408889634;
+    const float beta = nbeta;
+    fetch(hr + kPrepWarps);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double y = __shfl_up_sync(0xffffffffu, G, o);
