@@ -50,26 +50,32 @@ int64_t ws_chunks(int batch, int seqlen, int packed) {
 
 template <int N>
 int launch_chunks(nssm::DeltaChunkParams& p, void* ws, cudaStream_t st) {
+  using L = nssm::ChunkSmem<N>;
   auto prep = nssm::delta_prep_kernel<N>;
-  auto walk = nssm::delta_chunk_kernel<N>;
   p.img = static_cast<unsigned char*>(ws);
   p.blk = p.img + (int64_t)p.chunks * p.s.G * nssm::kImgBytes<N>;
-  const int smem = nssm::ChunkSmem<N>::bytes(p.stages, p.heads);
-  cudaError_t e = cudaFuncSetAttribute(prep, cudaFuncAttributeMaxDynamicSharedMemorySize, nssm::PrepSmem<N>::kBytes);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(walk, cudaFuncAttributeMaxDynamicSharedMemorySize, nssm::ChunkSmem<N>::bytes(nssm::kChunkStages, nssm::kWarps));
+  const dim3 grid(p.s.G * p.tile_groups, p.s.B);
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const bool help = (int64_t)grid.x * grid.y <= sms;
+  auto walk = help ? nssm::delta_chunk_kernel<N, true> : nssm::delta_chunk_kernel<N, false>;
+  p.stages = p.heads == 1 || (help && p.heads == 2) ? 4 : 3;   // as many as the CTAs of an SM have room for
+  const int smem = L::bytes(p.stages, p.heads, help);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(prep, cudaFuncAttributeMaxDynamicSharedMemorySize, nssm::PrepSmem<N>::kBytes);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(walk, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(walk, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+  static_assert(L::bytes(4, 2, true) <= 200 * 1024 && L::bytes(3, nssm::kWarps, true) <= 200 * 1024, "shared memory");
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(NSSM_ERR_CUDA, "delta scan: %s", cudaGetErrorString(e));
   }
-  const dim3 grid(p.s.G * p.tile_groups, p.s.B), block(nssm::kWarps * 32);
   if (p.chunks > 0) {
     prep<<<dim3(p.chunks, p.s.G), nssm::kPrepThreads, nssm::PrepSmem<N>::kBytes, st>>>(p);
     const int rc = launched("delta_prep_kernel");
     if (rc) return rc;
   }
-  walk<<<grid, block, smem, st>>>(p);
+  walk<<<grid, nssm::kWarps * (help ? 64 : 32), smem, st>>>(p);
   return launched("delta_chunk_kernel");
 }
 
@@ -180,7 +186,6 @@ int nssm_delta_scan(const nssm_delta_scan_args* a, void* stream) {
   c.tile_groups = (a->nheads / a->ngroups * c.tiles + nssm::kWarps - 1) / nssm::kWarps;
   // four tiles from a multiple of four on lie in one or two heads of two tiles or more
   c.heads = c.tiles == 1 ? nssm::kWarps : c.tiles % nssm::kWarps ? 2 : 1;
-  c.stages = c.heads == 1 ? 4 : 3;   // as many as two CTAs of an SM have room for
   return a->dstate == 64 ? launch_chunks<64>(c, a->workspace, st) : launch_chunks<128>(c, a->workspace, st);
 }
 

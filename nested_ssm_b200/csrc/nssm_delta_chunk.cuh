@@ -397,8 +397,12 @@ constexpr int kVBytes = kC * kVPitch;
 template <int N>
 struct ChunkSmem {
   static __host__ __device__ constexpr int stage(int heads) { return (kImgBytes<N> + heads * kBlkBytes + 127) / 128 * 128; }
-  static __host__ __device__ constexpr int bytes(int stages, int heads) {
-    return stages * stage(heads) + kWarps * 2 * kVBytes;
+  // what a tile's warp hands to its helper for a chunk: 16-column fragments of S's first pieces, then
+  // the fragments of u~ and two scales; two chunks, then the helper's y tile
+  static constexpr int kHand = (N / 16 + kSteps) * 512 + 16;
+  static constexpr int kHelp = 2 * kHand + kVBytes;
+  static __host__ __device__ constexpr int bytes(int stages, int heads, bool help) {
+    return stages * stage(heads) + kWarps * (2 * kVBytes + (help ? kHelp : 0));
   }
 };
 
@@ -406,12 +410,18 @@ struct ChunkSmem {
 // belong to different heads.  Two CTAs (up to 255 registers a thread) put two warps on each quarter
 // of an SM, whatever the headdim; three CTAs of 168 registers were slower (844 against 819 us for
 // 8 x 2048 tokens of 128 heads of 80).
-template <int N>
-__global__ void __launch_bounds__(kWarps * 32, 2) delta_chunk_kernel(const DeltaChunkParams p) {
+//
+// HELP: where a call has no more CTAs than SMs, one warp on each quarter would do all of a chunk's
+// work in turn.  y is not part of the chain from chunk to chunk, so a second warp computes it from
+// the operands that the first one hands over (one prompt of 4096 tokens, 32 heads of
+// 128: the walk 205 against 244 us).
+template <int N, bool HELP>
+__global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta_chunk_kernel(const DeltaChunkParams p) {
   using L = ChunkSmem<N>;
   extern __shared__ __align__(128) unsigned char sm[];
-  __shared__ uint64_t full[kChunkStages], empty[kChunkStages];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ uint64_t full[kChunkStages], empty[kChunkStages], handed[kWarps][2], taken[kWarps][2];
+  const int tid = threadIdx.x, lane = tid & 31, role = tid >> 5, warp = role % kWarps;   // warp: the tile in the CTA
+  const bool helper = HELP && role >= kWarps;
   const int grp = blockIdx.x / p.tile_groups, tg = blockIdx.x - grp * p.tile_groups, s = blockIdx.y;
   int batch, t0, len;
   if (!delta_seq(p.s, s, &batch, &t0, &len)) {
@@ -427,8 +437,13 @@ __global__ void __launch_bounds__(kWarps * 32, 2) delta_chunk_kernel(const Delta
   if (tid == 0) {
     for (int i = 0; i < kChunkStages; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], warps);
+      mbar_init(&empty[i], HELP ? 2 * warps : warps);
     }
+    if (HELP)
+      for (int i = 0; i < 2 * kWarps; ++i) {
+        mbar_init(&handed[0][0] + i, 1);
+        mbar_init(&taken[0][0] + i, 1);
+      }
     fence_mbar_init();
   }
   __syncthreads();
@@ -463,6 +478,92 @@ __global__ void __launch_bounds__(kWarps * 32, 2) delta_chunk_kernel(const Delta
            r < nt);
     }
   };
+
+  // y of chunk c, from O in the scale inv: through a tile in shared memory, then 16 bytes a lane
+  auto finish = [&](float (*O)[4], const float* fac, float inv, uint32_t yt, int c) {
+#pragma unroll
+    for (int j = 0; j < kTiles; j += 2) {
+      uint32_t w[4];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float2 k = *reinterpret_cast<const float2*>(fac + 3 * kC + 8 * (j + x) + (lane & 3) * 2);
+        k.x *= inv;
+        k.y *= inv;
+        w[2 * x] = bf2(k.x * O[j + x][0], k.y * O[j + x][1]);
+        w[2 * x + 1] = bf2(k.x * O[j + x][2], k.y * O[j + x][3]);
+      }
+      stsm4t(yt + (8 * (j + (lane >> 4)) + (lane & 7)) * kVPitch + ((lane >> 3) & 1) * 16, w[0], w[1], w[2], w[3]);
+    }
+    __syncwarp();
+    const int nt = min(kC, len - c * kC);
+    __nv_bfloat16* gy = p.s.y + batch * p.s.y_b + ((int64_t)t0 + (int64_t)c * kC) * p.s.y_t + h * p.s.P + row_h;
+#pragma unroll
+    for (int i = 0; i < kC / 16; ++i) {
+      const int r = i * 16 + (lane >> 1), x = lane & 1;
+      if (r < nt)
+        *reinterpret_cast<uint4*>(gy + (int64_t)r * p.s.y_t + x * 8) =
+            *reinterpret_cast<const uint4*>(sm + (yt - base) + r * kVPitch + x * 16);
+    }
+    __syncwarp();
+  };
+  unsigned char* hand = sm + stages * stage + kWarps * 2 * kVBytes + warp * L::kHelp;
+  if constexpr (HELP) {
+    if (helper) {
+      bool ok = true;
+      int si = 0, phase = 0;
+      for (int c = 0; c < nchunk; ++c) {
+        if (c && ++si == stages) {
+          si = 0;
+          phase ^= 1;
+        }
+        ok = warp_wait(&full[si], phase, p.s.polls);
+        ok = ok && warp_wait(&handed[warp][c & 1], (c >> 1) & 1, p.s.polls);
+        if (!ok) break;
+        const uint32_t st = base + si * stage;
+        const unsigned char* blk = sm + si * stage + kImgBytes<N> + (hr - h0) * kBlkBytes;
+        const float* fac = reinterpret_cast<const float*>(blk + kBlkF);
+        const unsigned char* in = hand + (c & 1) * L::kHand;
+        float O[kTiles][4] = {};
+#pragma unroll
+        for (int ks = 0; ks < N / 16; ++ks) {
+          const uint4 q = *reinterpret_cast<const uint4*>(in + ks * 512 + lane * 16);
+          const uint32_t a[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int j = 0; j < kTiles; j += 2) {
+            uint32_t d[4];
+            ldsm4(d, st + kC * N * 2 + tile_off<N>(8 * (j + (lane >> 4)) + (lane & 7), 2 * ks + ((lane >> 3) & 1)));
+            mma16816(O[j], a, d[0], d[1]);
+            mma16816(O[j + 1], a, d[2], d[3]);
+          }
+        }
+        const float2 sc = *reinterpret_cast<const float2*>(in + (N / 16 + kSteps) * 512);
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) {
+          float2 eg = *reinterpret_cast<const float2*>(fac + 2 * kC + 8 * j + (lane & 3) * 2);
+          eg.x *= sc.x;
+          eg.y *= sc.x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) O[j][e] *= e & 1 ? eg.y : eg.x;
+        }
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks) {
+          const uint4 q = *reinterpret_cast<const uint4*>(in + (N / 16 + ks) * 512 + lane * 16);
+          const uint32_t a[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int j = 2 * ks; j < kTiles; ++j) {
+            const uint2 b = *reinterpret_cast<const uint2*>(blk + lane * 8 + kBlkM + frag_index(j, ks) * kFragBytes);
+            mma16816(O[j], a, b.x, b.y);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&taken[warp][c & 1]);
+        finish(O, fac, sc.y, sm32(hand) + 2 * L::kHand, c);
+        if (lane == 0) mbar_arrive(&empty[si]);
+      }
+      if (!ok && lane == 0 && p.s.status) atomicOr(p.s.status, STATUS_TIMEOUT);
+      return;
+    }
+  }
 
   // S: tile t, element e: row lane / 4 + 8 (e / 2), column 8 t + 2 (lane % 4) + e % 2
   float S[N / 8][4];
@@ -517,6 +618,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) delta_chunk_kernel(const Delta
     const uint32_t st = base + si * stage, vt = vbase + (c & 1) * kVBytes;
     const unsigned char* blk = sm + si * stage + kImgBytes<N> + (hr - h0) * kBlkBytes;
     const float* fac = reinterpret_cast<const float*>(blk + kBlkF);
+    unsigned char* out = hand + (c & 1) * L::kHand;
+    if (HELP && c >= 2) {     // the helper is through the chunk before the last
+      ok = warp_wait(&taken[warp][c & 1], ((c >> 1) - 1) & 1, p.s.polls);
+      if (!ok) break;
+    }
     // P = S K^T and O = S Q^T (state rows x tokens)
     float Pm[kTiles][4] = {}, O[kTiles][4] = {};
     __half2 smax = __float2half2_rn(0.0f);
@@ -534,18 +640,22 @@ __global__ void __launch_bounds__(kWarps * 32, 2) delta_chunk_kernel(const Delta
       for (int j = 0; j < kTiles; j += 2) {
         const uint32_t off = tile_off<N>(8 * (j + (lane >> 4)) + (lane & 7), 2 * ks + ((lane >> 3) & 1));
         ldsm4(b[j / 2], st + off);
-        ldsm4(d[j / 2], st + kC * N * 2 + off);
+        if (!HELP) ldsm4(d[j / 2], st + kC * N * 2 + off);
       }
       // products into one accumulator are apart by a round over the tiles; the next pieces between them
 #pragma unroll
       for (int x = 0; x < 3 * kTiles; ++x) {
         const int j = x % kTiles, r = x / kTiles;
-        if (r == 1)
-          mma16816(O[j], sa[ks & 1][0], d[j / 2][2 * (j & 1)], d[j / 2][2 * (j & 1) + 1]);
-        else
+        if (r == 1) {
+          if (!HELP) mma16816(O[j], sa[ks & 1][0], d[j / 2][2 * (j & 1)], d[j / 2][2 * (j & 1) + 1]);
+        } else {
           mma16816(Pm[j], sa[ks & 1][r / 2], b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
+        }
         if (x % 3 == 0 && ks + 1 < N / 16) pieces(ks + 1, x / 3);
       }
+      if (HELP)
+        *reinterpret_cast<uint4*>(out + ks * 512 + lane * 16) =
+            make_uint4(sa[ks & 1][0][0], sa[ks & 1][0][1], sa[ks & 1][0][2], sa[ks & 1][0][3]);
     }
     // r = beta (v - e^G S k), in place
     float rmax = 0.0f;
@@ -607,6 +717,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) delta_chunk_kernel(const Delta
 #pragma unroll
       for (int e = 0; e < 4; ++e) S[t][e] *= es;
     // O = 2^-12 e^G S q^ + M u~
+    if (!HELP)
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) {
       float2 eg = *reinterpret_cast<const float2*>(fac + 2 * kC + 8 * j + (lane & 3) * 2);
@@ -626,10 +737,18 @@ __global__ void __launch_bounds__(kWarps * 32, 2) delta_chunk_kernel(const Delta
         a[e] = hf2(x, y);
         split2(et.x * x, et.y * y, au[0][e], au[1][e]);
       }
+      if (HELP)
+        *reinterpret_cast<uint4*>(out + (N / 16 + ks) * 512 + lane * 16) = make_uint4(a[0], a[1], a[2], a[3]);
+      else
 #pragma unroll
       for (int j = 2 * ks; j < kTiles; ++j) {
         const uint2 b = *reinterpret_cast<const uint2*>(tf + kBlkM + frag_index(j, ks) * kFragBytes);
         mma16816(O[j], a, b.x, b.y);
+      }
+      if (HELP && ks == kSteps - 1) {
+        if (lane == 0) *reinterpret_cast<float2*>(out + (N / 16 + kSteps) * 512) = make_float2(os, su.inv);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&handed[warp][c & 1]);
       }
 #pragma unroll
       for (int t = 0; t < N / 8; t += 4) {
@@ -643,30 +762,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) delta_chunk_kernel(const Delta
           for (int x = 0; x < 4; ++x) mma16816(S[t + x], au[i], b[x / 2][2 * (x & 1)], b[x / 2][2 * (x & 1) + 1]);
       }
     }
-    // y: through the V tile, then 16 bytes a lane
-#pragma unroll
-    for (int j = 0; j < kTiles; j += 2) {
-      uint32_t w[4];
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        float2 k = *reinterpret_cast<const float2*>(fac + 3 * kC + 8 * (j + x) + (lane & 3) * 2);
-        k.x *= su.inv;
-        k.y *= su.inv;
-        w[2 * x] = bf2(k.x * O[j + x][0], k.y * O[j + x][1]);
-        w[2 * x + 1] = bf2(k.x * O[j + x][2], k.y * O[j + x][3]);
-      }
-      stsm4t(vt + (8 * (j + (lane >> 4)) + (lane & 7)) * kVPitch + ((lane >> 3) & 1) * 16, w[0], w[1], w[2], w[3]);
-    }
-    __syncwarp();
-    const int nt = min(kC, len - c * kC);
-    __nv_bfloat16* gy = p.s.y + batch * p.s.y_b + ((int64_t)t0 + (int64_t)c * kC) * p.s.y_t + h * p.s.P + row_h;
-#pragma unroll
-    for (int i = 0; i < kC / 16; ++i) {
-      const int r = i * 16 + (lane >> 1), x = lane & 1;
-      if (r < nt)
-        *reinterpret_cast<uint4*>(gy + (int64_t)r * p.s.y_t + x * 8) =
-            *reinterpret_cast<const uint4*>(sm + (vt - base) + r * kVPitch + x * 16);
-    }
+    if (!HELP) finish(O, fac, su.inv, vt, c);
     __syncwarp();
     if (lane == 0) mbar_arrive(&empty[si]);
   }

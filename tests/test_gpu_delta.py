@@ -465,3 +465,27 @@ def test_a_value_that_is_not_finite_stays_in_its_sequence_and_block():
     _check_y(y[0, :64], yr[0, :64])                      # blocks of 32 tokens before it
     assert bool(torch.isnan(y[0, 70:, 1, 3]).all())
     _check_y(y[0, :, 0], yr[0, :, 0])                    # the other head
+
+
+@pytest.mark.parametrize("b,T,H,G,P,N,packed", [
+    (24, 70, 8, 2, 80, 128, False),
+    (80, 100, 8, 2, 16, 64, False),       # four heads in a CTA
+    (40, 200, 16, 4, 128, 128, True),
+    (50, 33, 12, 4, 48, 64, True),
+])
+def test_scan_of_more_work_than_sms(b, T, H, G, P, N, packed):
+    """Enough sequences and heads that CTAs share SMs: the other form of the walk."""
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    d = _inputs(b, T, H, G, P, N, seed=b + T)
+    x = [d[n] for n in ("q", "k", "v", "g", "beta")]
+    yr, Sr = OD.gated_delta_scan(*x, S0=d["s0"])
+    cu = None
+    if packed:
+        x = [t.reshape(1, b * T, *t.shape[2:]) for t in x]
+        cu = torch.arange(0, b * T + 1, T, dtype=torch.int32, device="cuda")
+    y, S = gated_delta_chunk_scan(*x, initial_states=d["s0"], cu_seqlens=cu, return_final_states=True)
+    _check_y(y.view(b, T, H, P), yr)
+    _check_state(S, Sr)
+    one = gated_delta_chunk_scan(*(d[n][:1] for n in ("q", "k", "v", "g", "beta")), initial_states=d["s0"][:1],
+                                 return_final_states=True)
+    assert torch.equal(one[0], y.view(b, T, H, P)[:1]) and torch.equal(one[1], S[:1])    # and the same values
