@@ -16,14 +16,15 @@
 // register file; on tcgen05 each of its four dependent products would cross tensor memory twice,
 // with the same conversions between, for a 128-row tile that most headdims do not fill.
 //
-// What bounds it: of 2 x 8192 tokens of 32 heads of 128 (531 us; input and output alone 63 us) the walk
-// takes 434 us, one warp on each quarter of 128 SMs, 3030 cycles a chunk, 1470 of them mma (184
-// products of 8 cycles a quarter).  Of 8 x 2048 tokens of 128 heads of 80 (942 us) it takes 757 us,
-// two warps a quarter, the tensor pipe 55 to 73 % busy.  Not kept: chunks of 64 (T costs four times
-// as much a chunk: 1703 against 937 us), bf16 operands in three pieces (316 products a chunk against
-// 184; two pieces leave 3.6e-6 in the state), splitting the columns of S over two or four warps (the
-// part of a chunk that is not split and the exchange take more than is won: 489 -> 619 us), V by one
-// small bulk copy a row (they cost the walk more than its arithmetic).
+// What bounds it.  Of 2 x 8192 tokens of 32 heads of 128 (492 us; input and output alone 63 us) the
+// walk takes 390: a chain of 256 chunks, one warp on each quarter of 128 SMs, 2700 cycles a chunk, of
+// them 1170 mma (146 products of 8 cycles a quarter; 38 more, with y, in the helper warp).  Of
+// 8 x 2048 tokens of 128 heads of 80 (933 us; 128 us) it takes 760: two warps a quarter, 184 products
+// a chunk, the tensor pipe 55 to 73 % busy, 4.3 waves of CTAs.  Not kept: chunks of 64 (T costs four
+// times as much a chunk: 1703 against 937 us), bf16 operands in three pieces (316 products a chunk
+// against 184; two pieces leave 3.6e-6 in the state), splitting the columns of S over two or four warps
+// (the part of a chunk that is not split and the exchange take more than is won: 489 -> 619 us), V by
+// one small bulk copy a row (they cost the walk more than its arithmetic).
 //
 // Precision.  The state is fp32, and its products are to be as good: an fp32 operand goes in as two
 // fp16 values (11 bits each, the second holds what the first leaves), scaled by a power of two that
