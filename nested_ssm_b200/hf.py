@@ -190,20 +190,29 @@ def _lean_prefill(self, input_states, cache_params, attention_mask):
     return self.out_proj(scan_output.to(self.out_proj.weight.dtype))
 
 
-def _follow_beams(layer, st) -> None:
-    """Let the pool's slots follow the rows of a cache layer when beam search reorders them."""
-    if getattr(layer, "_nssm", None) is st:
-        return
-    rows_of_cache = layer.reorder_cache
+class _FollowBeams:
+    """A cache layer's ``reorder_cache``: the rows of the cache, then the pool's slots.  A deep copy of the
+    layer gets one of its own for the same pool."""
 
-    def reorder_cache(beam_idx):
-        rows_of_cache(beam_idx)
+    def __init__(self, layer, st):
+        self.layer, self.st = layer, st
+
+    def __call__(self, beam_idx):
+        type(self.layer).reorder_cache(self.layer, beam_idx)
+        st = self.st
         slots = st["slots"]
         if st["draft"] is not None:
             reorder_slots(StateBuffers([st["draft"]]), slots, beam_idx.to(slots.device))
         st["slots"] = reorder_slots(st["pool"], slots, beam_idx.to(slots.device))
 
-    layer._nssm, layer.reorder_cache = st, reorder_cache
+    def __deepcopy__(self, memo):
+        return _FollowBeams(memo.get(id(self.layer), self.layer), self.st)
+
+
+def _follow_beams(layer, st) -> None:
+    """Let the pool's slots follow the rows of a cache layer when beam search reorders them."""
+    if hasattr(type(layer), "reorder_cache"):
+        layer.reorder_cache = _FollowBeams(layer, st)
 
 
 def _dispatch(self, input_states, cache_params=None, attention_mask=None):

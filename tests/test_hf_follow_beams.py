@@ -1,0 +1,51 @@
+"""The hook that lets the pool's slots follow a cache layer's rows (host logic, CPU)."""
+import copy
+
+import torch
+
+from nested_ssm_b200 import hf
+
+
+class Layer:
+    def __init__(self):
+        self.rows = torch.arange(4)
+
+    def reorder_cache(self, beam_idx):
+        self.rows = self.rows[beam_idx]
+
+
+def _state(calls, monkeypatch):
+    def reorder(buffers, slots, parents):
+        calls.append((buffers, slots.tolist(), parents.tolist()))
+        return slots[parents]
+
+    monkeypatch.setattr(hf, "reorder_slots", reorder)
+    return {"pool": "pool", "slots": torch.tensor([3, 1, 0, 2]), "draft": None}
+
+
+def test_rows_and_slots_are_reordered_once_per_call(monkeypatch):
+    calls = []
+    layer, st = Layer(), _state(calls, monkeypatch)
+    hf._follow_beams(layer, st)
+    hf._follow_beams(layer, st)           # a second prefill on the same cache
+    layer.reorder_cache(torch.tensor([1, 1, 2, 0]))
+    assert layer.rows.tolist() == [1, 1, 2, 0] and st["slots"].tolist() == [1, 1, 0, 3]
+    assert calls == [("pool", [3, 1, 0, 2], [1, 1, 2, 0])]
+
+
+def test_a_deep_copy_reorders_its_own_rows(monkeypatch):
+    layer, st = Layer(), _state([], monkeypatch)
+    hf._follow_beams(layer, st)
+    other = copy.deepcopy([layer])[0]
+    other.reorder_cache(torch.tensor([3, 2, 1, 0]))
+    assert other.rows.tolist() == [3, 2, 1, 0] and layer.rows.tolist() == [0, 1, 2, 3]
+    assert other.reorder_cache.st is st
+
+
+def test_a_layer_without_rows_to_reorder_is_left_alone():
+    class Plain:
+        pass
+
+    layer = Plain()
+    hf._follow_beams(layer, {})
+    assert not hasattr(layer, "reorder_cache")
