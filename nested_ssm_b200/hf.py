@@ -28,6 +28,7 @@ cold read, ring or flush.
 from __future__ import annotations
 
 import math
+import weakref
 
 import torch
 import torch.nn.functional as F
@@ -195,18 +196,19 @@ class _FollowBeams:
     layer gets one of its own for the same pool."""
 
     def __init__(self, layer, st):
-        self.layer, self.st = layer, st
+        self.layer, self.st = weakref.ref(layer), st     # (the layer holds this: no cycle)
 
     def __call__(self, beam_idx):
-        type(self.layer).reorder_cache(self.layer, beam_idx)
-        st = self.st
+        layer, st = self.layer(), self.st
+        type(layer).reorder_cache(layer, beam_idx)
         slots = st["slots"]
         if st["draft"] is not None:
             reorder_slots(StateBuffers([st["draft"]]), slots, beam_idx.to(slots.device))
         st["slots"] = reorder_slots(st["pool"], slots, beam_idx.to(slots.device))
 
     def __deepcopy__(self, memo):
-        return _FollowBeams(memo.get(id(self.layer), self.layer), self.st)
+        layer = self.layer()
+        return _FollowBeams(memo.get(id(layer), layer), self.st)
 
 
 def _follow_beams(layer, st) -> None:

@@ -49,3 +49,17 @@ def test_a_layer_without_rows_to_reorder_is_left_alone():
     layer = Plain()
     hf._follow_beams(layer, {})
     assert not hasattr(layer, "reorder_cache")
+
+
+def test_a_layer_goes_with_its_last_reference(monkeypatch):
+    import gc
+    import weakref
+    layer, st = Layer(), _state([], monkeypatch)
+    hf._follow_beams(layer, st)
+    gc.disable()
+    try:
+        gone = weakref.ref(layer)
+        del layer
+        assert gone() is None
+    finally:
+        gc.enable()
