@@ -614,6 +614,7 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
     if (c + 1 < nchunk) load_v(c + 1);
     cp_commit();
     cp_wait<1>();
+    __syncwarp();      // every lane's part of V is there
     ok = warp_wait(&full[si], phase, p.s.polls) && ok;
     if (!ok) break;
     const uint32_t st = base + si * stage, vt = vbase + (c & 1) * kVBytes;
