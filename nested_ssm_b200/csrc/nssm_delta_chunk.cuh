@@ -390,6 +390,7 @@ __global__ void __launch_bounds__(kPrepThreads, 7) delta_prep_kernel(const Delta
 // two chunks ago: a chunk's copies take about as long as its work, and the warp that issues them
 // should not wait for the slowest warp's last chunk.
 constexpr int kChunkStages = 4;
+constexpr int kSorted = 128;  // packed sequences that a CTA ranks by their length
 constexpr int kWarps = 4;     // 16-row tiles of a CTA, one on each quarter of an SM
 // A warp's own V tile: 32 tokens of 16 values, at a pitch that puts 8 rows into 8 bank groups; the
 // next chunk's lies beside it.  y leaves through it.
@@ -423,8 +424,22 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
   __shared__ uint64_t full[kChunkStages], empty[kChunkStages], handed[kWarps][2], taken[kWarps][2];
   const int tid = threadIdx.x, lane = tid & 31, role = tid >> 5, warp = role % kWarps;   // warp: the tile in the CTA
   const bool helper = HELP && role >= kWarps;
-  const int grp = blockIdx.x / p.tile_groups, tg = blockIdx.x - grp * p.tile_groups, s = blockIdx.y;
-  int batch, t0, len;
+  const int grp = blockIdx.x / p.tile_groups, tg = blockIdx.x - grp * p.tile_groups;
+  int s = blockIdx.y, batch, t0, len;
+  if (p.s.cu && p.s.B > 1 && p.s.B <= kSorted) {
+    // the longest sequences first: CTAs start in this order, and the last ones to start should be short
+    // (24 prompts of 35 to 700 tokens, 32 heads of 128: 206 against 231 us)
+    __shared__ int lens[kSorted], chosen;
+    for (int i = tid; i < p.s.B; i += blockDim.x) lens[i] = delta_seq(p.s, i, &batch, &t0, &len) ? len : 0;
+    __syncthreads();
+    for (int i = tid; i < p.s.B; i += blockDim.x) {
+      int rank = 0;
+      for (int j = 0; j < p.s.B; ++j) rank += lens[j] > lens[i] || (lens[j] == lens[i] && j < i);
+      if (rank == (int)blockIdx.y) chosen = i;
+    }
+    __syncthreads();
+    s = chosen;
+  }
   if (!delta_seq(p.s, s, &batch, &t0, &len)) {
     if (p.s.status && blockIdx.x == 0 && tid == 0) atomicOr(p.s.status, STATUS_CONFLICT);
     return;
