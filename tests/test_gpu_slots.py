@@ -255,3 +255,58 @@ def test_two_replayed_graphs_and_another_stream():
     new, moves = OD.compact_plan([5, 36, 0], -1)
     _same(t, _apply(want, moves))
     assert o2.tolist() == new
+
+
+def test_nothing_to_do():
+    """Empty lists and batches in every call."""
+    from nested_ssm_b200 import (StateBuffers, beam_select, clear_slots, compact_slots, copy_slots, gated_delta_chunk_scan,
+                                 reorder_slots)
+    t = [torch.randn(2, 5, 33, device="cuda")]
+    bufs = StateBuffers(t, slot_dim=1)
+    want = t[0].clone()
+    none = _i32([])
+    copy_slots(bufs, none, none)
+    clear_slots(bufs, none)
+    assert compact_slots(bufs, none).shape == (0,)
+    assert reorder_slots(bufs, none.view(0, 4), none.view(0, 4)).shape == (0, 4)
+    assert compact_slots(bufs, _i32([-1, -1])).tolist() == [-1, -1]
+    assert reorder_slots(bufs, _i32([[-1, -1]]), _i32([[0, 1]])).tolist() == [[-1, -1]]
+    assert torch.equal(t[0], want)
+    bufs.check_status()
+    s, p, k = beam_select(torch.zeros(0, 3, 7, device="cuda"), torch.zeros(0, 3, device="cuda"), 2)
+    assert s.shape == p.shape == k.shape == (0, 2)
+    z = lambda *sh: torch.zeros(*sh, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    y, S = gated_delta_chunk_scan(z(0, 9, 2, 64), z(0, 9, 2, 64), z(0, 9, 4, 32), z(0, 9, 4), z(0, 9, 4), return_final_states=True)
+    assert y.shape == (0, 9, 4, 32) and S.shape == (0, 4, 32, 64)
+    y, S = gated_delta_chunk_scan(z(1, 0, 2, 64), z(1, 0, 2, 64), z(1, 0, 4, 32), z(1, 0, 4), z(1, 0, 4),
+                                  cu_seqlens=_i32([0, 0, 0]), return_final_states=True)
+    assert y.shape == (1, 0, 4, 32) and S.shape == (2, 4, 32, 64) and float(S.abs().max()) == 0
+
+
+def test_two_calls_at_once_on_two_streams():
+    """Calls on two streams share no workspace: moves of other slots, and prompts, side by side."""
+    from nested_ssm_b200 import StateBuffers, copy_slots, gated_delta_chunk_scan, beam_select
+    t = [torch.randn(3, 64, 4, 64, 64, device="cuda")]
+    bufs = StateBuffers(t, slot_dim=1)
+    want = t[0].clone()
+    want[:, 16:32], want[:, 48:64] = want[:, 0:16].clone(), want[:, 32:48].clone()
+    g = torch.Generator(device="cuda").manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    x = [(r(2, 150, 2, 64) / 8).bfloat16(), (r(2, 150, 2, 64) / 8).bfloat16(), r(2, 150, 4, 48).bfloat16(), -r(2, 150, 4).abs(),
+         torch.sigmoid(r(2, 150, 4))]
+    logits, scores = r(4, 4, 20000), r(4, 4)
+    ref = gated_delta_chunk_scan(*x), beam_select(logits, scores)
+    lists = [(_i32(range(0, 16)), _i32(range(16, 32))), (_i32(range(32, 48)), _i32(range(48, 64)))]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for st, (a, b) in zip(streams, lists):
+            with torch.cuda.stream(st):
+                copy_slots(bufs, a, b)
+                got.append((gated_delta_chunk_scan(*x), beam_select(logits, scores)))
+    torch.cuda.synchronize()
+    assert torch.equal(t[0], want)
+    for y, sel in got:
+        assert torch.equal(y, ref[0]) and all(torch.equal(m, n) for m, n in zip(sel, ref[1]))
+    bufs.check_status()
