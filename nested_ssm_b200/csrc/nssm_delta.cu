@@ -6,6 +6,8 @@
 
 namespace nssm_host {
 int fail(int code, const char* fmt, ...);
+uint32_t wait_polls();   // nssm_set_wait_polls
+int inject_stuck();      // nssm_test_inject_stuck_copy
 }
 
 namespace {
@@ -172,7 +174,7 @@ int nssm_delta_scan(const nssm_delta_scan_args* a, void* stream) {
   p.y = static_cast<__nv_bfloat16*>(a->y); p.y_b = a->y_stride_b; p.y_t = a->y_stride_t;
   p.fin = a->final_states; p.fin_b = a->final_stride_b;
   p.status = a->status;
-  p.polls = nssm::kSpinLimit;
+  p.polls = nssm_host::wait_polls();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const size_t need = nssm_delta_scan_workspace_bytes(a->batch, a->seqlen, a->nheads, a->ngroups, a->dstate,
                                                     a->cu_seqlens != nullptr);
@@ -180,6 +182,7 @@ int nssm_delta_scan(const nssm_delta_scan_args* a, void* stream) {
     return fail(NSSM_ERR_INVALID, "a 32-byte aligned workspace of %zu bytes is needed (got %zu)", need, a->workspace_bytes);
   nssm::DeltaChunkParams c{};
   c.s = p;
+  c.stuck = nssm_host::inject_stuck();
   c.chunks = (int)ws_chunks(a->batch, a->seqlen, a->cu_seqlens != nullptr);
   c.per_seq = (a->seqlen + kC - 1) / kC;
   c.tiles = a->headdim / 16;

@@ -69,6 +69,7 @@ struct DeltaChunkParams {
   int tile_groups;       // CTAs per key group and sequence
   int heads;             // heads of a CTA's tiles at most
   int stages;            // chunks in shared memory
+  int stuck;             // failure injection (tests only): CTA 0's first copies never complete
 };
 
 __device__ __forceinline__ uint32_t bf2(float lo, float hi) {
@@ -477,7 +478,8 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
     unsigned char* st = sm + (c % stages) * stage;
     uint64_t* bar = &full[c % stages];
     if (lane == 0) {
-      mbar_expect_tx(bar, kImgBytes<N> + nh * kBlkBytes);
+      const bool stuck = p.stuck && c == 0 && blockIdx.x == 0 && blockIdx.y == 0;
+      mbar_expect_tx(bar, kImgBytes<N> + nh * kBlkBytes + (stuck ? 16 : 0));
       bulk_g2s(st, gimg + (int64_t)c * p.s.G * kImgBytes<N>, kImgBytes<N>, bar);
       bulk_g2s(st + kImgBytes<N>, gblk + (int64_t)c * p.s.H * kBlkBytes, nh * kBlkBytes, bar);
     }

@@ -489,3 +489,28 @@ def test_scan_of_more_work_than_sms(b, T, H, G, P, N, packed):
     one = gated_delta_chunk_scan(*(d[n][:1] for n in ("q", "k", "v", "g", "beta")), initial_states=d["s0"][:1],
                                  return_final_states=True)
     assert torch.equal(one[0], y.view(b, T, H, P)[:1]) and torch.equal(one[1], S[:1])    # and the same values
+
+
+@pytest.mark.parametrize("b,T", [(1, 100), (80, 40)])
+def test_a_copy_that_never_completes_times_out(b, T):
+    """The injected stuck copy (the first CTA announces 16 bytes more than arrive): its waits run out, the
+    call returns with bit 1 set, other sequences are as ever and the next call is right."""
+    from nested_ssm_b200 import _lib, gated_delta_chunk_scan
+    lib = _lib.load()
+    H, G, P, N = 8, 2, 64, 128
+    d = _inputs(b, T, H, G, P, N, seed=25)
+    x = [d[n] for n in ("q", "k", "v", "g", "beta")]
+    want = gated_delta_chunk_scan(*x, return_final_states=True)
+    torch.cuda.synchronize()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    polls, stuck = lib.nssm_set_wait_polls(4096), lib.nssm_test_inject_stuck_copy(1)
+    try:
+        got = gated_delta_chunk_scan(*x, return_final_states=True, status=status)
+        torch.cuda.synchronize()
+    finally:
+        lib.nssm_test_inject_stuck_copy(stuck)
+        lib.nssm_set_wait_polls(polls)
+    assert int(status) == 2
+    assert torch.equal(got[0][1:], want[0][1:]) and torch.equal(got[1][1:], want[1][1:])
+    again = gated_delta_chunk_scan(*x, return_final_states=True, status=status.zero_())
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1]) and int(status) == 0
