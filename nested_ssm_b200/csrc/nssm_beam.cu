@@ -220,9 +220,10 @@ __device__ __noinline__ int beam_exact(BeamRow<BF16> r, int step0, int steps, in
 // A part of a row, a step of kBeamThreads * kVecs 16-byte pieces at a time, the next one's loads in
 // flight; the max, the sum and the candidates of a step all come from one read into registers.
 // Candidates are the values that reach a lower bound of the nout-th best, the nout-th best of a
-// few maxima of each warp in the first step, so later steps need no barrier; a step only notes
-// the pieces that hold any, which are read again and ranked at the end.  Where the bound lets
-// through too many (sorted or constant logits), beam_exact reads the part again.
+// few maxima of each warp in the first step, so most steps need no barrier; a step only notes
+// the pieces that hold any, which are read again and ranked after a few steps (the bound then rises)
+// and at the end.  Where the bound lets through too many (sorted or constant logits), beam_exact
+// reads the part again.
 template <bool BF16>
 __global__ void __launch_bounds__(kBeamThreads, BF16 ? 3 : 4) beam_scan_kernel(const BeamParams p) {
   using Row = BeamRow<BF16>;
@@ -246,7 +247,36 @@ __global__ void __launch_bounds__(kBeamThreads, BF16 ? 3 : 4) beam_scan_kernel(c
   const int steps = max(0, min(p.steps, (p.V + r.lead + Row::kStep - 1) / Row::kStep - step0));
   float m = kNegInf, sum = 0.0f;                        // this thread's running maximum and sum
   float tau = kNegInf;
+  int have = 0;
+  bool many = false;                                    // more candidates than the list is for
   if (tid == 0) count = pieces = 0;
+  // the values of the noted pieces that reach the bound go to the list, read again; how many it has
+  auto gather = [&]() {
+    __syncthreads();
+    const int np = pieces;
+    if (np <= kPieces)
+      for (int i = tid; i < np; i += kBeamThreads) {
+        uint4 one;
+        float v[E], top;
+        r.load(plist[i], one);
+        r.values(one, v, top);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int tk = plist[i] + e;
+          if (v[e] >= tau && tk >= 0 && tk < p.V) {
+            const int at = atomicAdd(&count, 1);
+            if (at < kCap) list[at] = key_of(v[e], tk);
+          }
+        }
+      }
+    __syncthreads();
+    const int found = np <= kPieces ? count : kCap + 1;
+    __syncthreads();
+    if (tid == 0) pieces = 0;
+    return found;
+  };
+  // ranking is quadratic in the list: beyond this beam_exact's shorter lists are the cheaper way
+  const int most = min(kCap, 256 + 6 * p.n);
   uint4 raw[kVecs];
   if (steps > 0) r.fetch(step0, raw);
   for (int st = step0; st < step0 + steps; ++st) {
@@ -277,37 +307,35 @@ __global__ void __launch_bounds__(kBeamThreads, BF16 ? 3 : 4) beam_scan_kernel(c
       tau = unorder32(bound);
       if (!(tau >= kNegInf)) tau = kNegInf;     // fewer values than that
     }
+    if (!many) {
 #pragma unroll
-    for (int c = 0; c < kVecs; ++c)
-      if (mxc[c] >= tau) {
-        const int at = atomicAdd(&pieces, 1);
-        if (at < kPieces) plist[at] = r.first(st, c);
-      }
-  }
-  __syncthreads();
-  const int np = pieces;
-  if (np <= kPieces)
-    for (int i = tid; i < np; i += kBeamThreads) {   // the values of the few pieces that reach the bound, read again
-      uint4 one;
-      float v[E], top;
-      r.load(plist[i], one);
-      r.values(one, v, top);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int tk = plist[i] + e;
-        if (v[e] >= tau && tk >= 0 && tk < p.V) {
-          const int at = atomicAdd(&count, 1);
-          if (at < kCap) list[at] = key_of(v[e], tk);
+      for (int c = 0; c < kVecs; ++c)
+        if (mxc[c] >= tau) {
+          const int at = atomicAdd(&pieces, 1);
+          if (at < kPieces) plist[at] = r.first(st, c);
+        }
+      // after 3, 7, 15 .. steps the nout-th best so far becomes the bound, so that a long part does not
+      // collect in proportion to its length
+      const int done = st - step0 + 1;
+      if (((done + 1) & done) == 0 && done > 2 && steps - done > 1) {
+        const int found = gather();
+        many = found > most;
+        if (!many) {
+          have = rank_list(list, found, p.n, cur);
+          for (int i = tid; i < have; i += kBeamThreads) list[i] = cur[i];
+          if (tid == 0) count = have;
+          if (have == p.n) tau = unorder32((uint32_t)(cur[p.n - 1] >> 32));
+          __syncthreads();
         }
       }
     }
-  __syncthreads();
-  // ranking is quadratic in the list: beyond this beam_exact's shorter lists are the cheaper way
-  const int found = count;
-  __syncthreads();
-  const int have = np <= kPieces && found <= max(512, 4 * p.n)
-                       ? rank_list(list, found, p.n, cur)
-                       : beam_exact<BF16>(r, step0, steps, p.n, sh, list, cur, &nth, &count);
+  }
+  if (!many) {
+    const int found = gather();
+    many = found > most;
+    if (!many) have = rank_list(list, found, p.n, cur);
+  }
+  if (many) have = beam_exact<BF16>(r, step0, steps, p.n, sh, list, cur, &nth, &count);
   uint64_t* out = p.cand + ((int64_t)row * p.splits + split) * p.n;
   for (int i = tid; i < p.n; i += kBeamThreads) out[i] = i < have ? cur[i] : 0;
   // the part's maximum and sum

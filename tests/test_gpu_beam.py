@@ -204,3 +204,25 @@ def test_beam_search_over_a_recurrent_layer():
         assert float((state[slots.long()].double() - ref).norm() / ref.norm()) <= 1e-5, step
         logits = (yr.reshape(b, K, -1) @ head).float()
     bufs.check_status()
+
+
+@pytest.mark.parametrize("n", [3, 16, 128])
+@pytest.mark.parametrize("order", ["random", "ascending", "descending", "few values"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_parts(n, order, dtype):
+    """So many rows that one CTA walks a whole row in many steps, the bound rising on the way: against the
+    sort for two of the prompts; every prompt has the same logits but for a shift that changes nothing."""
+    from nested_ssm_b200 import beam_select
+    b, K, V = 56, 16, 70001
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = {"random": lambda: 3 * torch.randn(K, V, generator=g, device="cuda"),
+         "ascending": lambda: torch.linspace(-20, 20, V, device="cuda").expand(K, V),
+         "descending": lambda: torch.linspace(20, -20, V, device="cuda").expand(K, V),
+         "few values": lambda: torch.randint(-2, 3, (K, V), generator=g, device="cuda").float()}[order]()
+    x = x.to(dtype)
+    s = -torch.rand(b, K, generator=g, device="cuda")
+    s[1:] = s[:1]
+    got = beam_select(x.expand(b, K, V), s, n)
+    _check([t[:1] for t in got], x[None], s[:1], n)
+    for t in got:
+        assert torch.equal(t, t[:1].expand_as(t))
