@@ -211,7 +211,7 @@ def test_beam_search_over_a_recurrent_layer():
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_long_parts(n, order, dtype):
     """So many rows that one CTA walks a whole row in many steps, the bound rising on the way: against the
-    sort for two of the prompts; every prompt has the same logits but for a shift that changes nothing."""
+    sort for one prompt; every prompt has the same logits and scores."""
     from nested_ssm_b200 import beam_select
     b, K, V = 56, 16, 70001
     g = torch.Generator(device="cuda").manual_seed(n)
