@@ -50,6 +50,8 @@ int64_t ws_chunks(int batch, int seqlen, int packed) {
   return packed ? (int64_t)seqlen / kC + batch : (int64_t)batch * ((seqlen + kC - 1) / kC);
 }
 
+constexpr int kMaxSmem = 227 * 1024 - 1024;    // of a walking CTA, beside its static 1 KB
+
 template <int N>
 int launch_chunks(nssm::DeltaChunkParams& p, void* ws, cudaStream_t st) {
   using L = nssm::ChunkSmem<N>;
@@ -65,9 +67,9 @@ int launch_chunks(nssm::DeltaChunkParams& p, void* ws, cudaStream_t st) {
   p.stages = p.heads == 1 || (help && p.heads == 2) ? 4 : 3;   // as many as the CTAs of an SM have room for
   const int smem = L::bytes(p.stages, p.heads, help);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(prep, cudaFuncAttributeMaxDynamicSharedMemorySize, nssm::PrepSmem<N>::kBytes);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(walk, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(walk, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(walk, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
-  static_assert(L::bytes(4, 2, true) <= 200 * 1024 && L::bytes(3, nssm::kWarps, true) <= 200 * 1024, "shared memory");
+  static_assert(L::bytes(4, 2, true) <= kMaxSmem && L::bytes(3, nssm::kWarps, true) <= kMaxSmem, "shared memory");
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(NSSM_ERR_CUDA, "delta scan: %s", cudaGetErrorString(e));

@@ -18,11 +18,11 @@
 //
 // What bounds it.  Of 2 x 8192 tokens of 32 heads of 128 (492 us; input and output alone 63 us) the
 // walk takes 390: a chain of 256 chunks, one warp on each quarter of 128 SMs, 2700 cycles a chunk, of
-// them 1170 mma (146 products of 8 cycles a quarter; 38 more, with y, in the helper warp).  Of
-// 8 x 2048 tokens of 128 heads of 80 (933 us; 128 us) it takes 760: two warps a quarter, 184 products
+// them 1170 mma (146 products of 8 cycles a quarter; 82 more, with y, in the helper warp).  Of
+// 8 x 2048 tokens of 128 heads of 80 (933 us; 128 us) it takes 760: two warps a quarter, 228 products
 // a chunk, the tensor pipe 55 to 73 % busy, 4.3 waves of CTAs.  Not kept: chunks of 64 (T costs four
 // times as much a chunk: 1703 against 937 us), bf16 operands in three pieces (316 products a chunk
-// against 184; two pieces leave 3.6e-6 in the state), splitting the columns of S over two or four warps
+// against 184 at the same precision of y; two pieces leave 3.6e-6 in the state), splitting the columns of S over two or four warps
 // (the part of a chunk that is not split and the exchange take more than is won: 489 -> 619 us), V by
 // one small bulk copy a row (they cost the walk more than its arithmetic).
 //
@@ -30,9 +30,10 @@
 // fp16 values (11 bits each, the second holds what the first leaves), scaled by a power of two that
 // keeps the warp's values below 2^15; what is left out is below 2^-22 of a value or 2^-25.  K and Q
 // (bf16) become fp16 exactly, each token scaled by its own power of two (elements below 2^-25 of the
-// token's largest lose bits).  T goes in as two pieces, so only products of two second pieces are
-// left out, 2^-22 of a product.  y is rounded to bf16 (2^-9): the operands of its own products are
-// single fp16 values (2^-12).
+// token's largest lose bits).  T, M and u go in as two pieces, so only products of two second pieces are
+// left out, 2^-22 of a product.  y is the fp32 sum rounded once to bf16 (single fp16 operands, 2^-12, in its
+// own products moved 3e-4 of it, and one value in thirty by a step; they take 504 against 557 us for 2 x 8192
+// tokens of 32 heads, 950 against 1086 for 8 x 2048 of 128).
 #pragma once
 
 #include <cuda_fp16.h>
@@ -50,11 +51,11 @@ constexpr int kSteps = kC / 16;
 constexpr int kFrags = 6, kFragBytes = 256;
 __host__ __device__ constexpr int frag_index(int nt, int ks) { return nt < 2 ? nt : 2 * nt - 2 + ks; }
 // With k = sk k^ and q = sq q^ (sk, sq powers of two per token), the walk works on u~ = sk u.
-// Workspace block of a (chunk, head): two pieces of sT sk T, then 2^-12 D (q^.k^), then per token
+// Workspace block of a (chunk, head): two pieces of sT sk T, two of 2^-12 D (q^.k^), then per token
 // beta, beta e^G sk, 2^-12 e^G, 2^12 scale sq, e^{G_C - G}, then 1 / sT and the largest of the
 // e^{G_C - G} and 1.
 constexpr int kBlkM = 2 * kFrags * kFragBytes;
-constexpr int kBlkF = kBlkM + kFrags * kFragBytes;
+constexpr int kBlkF = kBlkM + 2 * kFrags * kFragBytes;
 constexpr int kBlkBytes = kBlkF + 5 * kC * 4 + 32;    // whole sectors
 // and of a (chunk, group): K^ and Q^ as the walk wants them in shared memory
 template <int N> constexpr int kImgBytes = 2 * kC * N * 2;
@@ -322,7 +323,7 @@ __global__ void __launch_bounds__(kPrepThreads, 7) delta_prep_kernel(const Delta
     unsigned char* frow = blk + (lane & 7) * 32;      // its 32 bytes of each fragment
 #pragma unroll
     for (int ks = 0; ks < kSteps; ++ks) {
-      uint32_t mw[8];
+      uint32_t mw[8], ml[8];
 #pragma unroll
       for (int j = 16 * ks; j < 16 * ks + 16; j += 4) {
         const float4 h4 = *reinterpret_cast<const float4*>(gh + j), l4 = *reinterpret_cast<const float4*>(gl + j);
@@ -341,11 +342,12 @@ __global__ void __launch_bounds__(kPrepThreads, 7) delta_prep_kernel(const Delta
         }
         // columns c, c + 1 are lane (c & 7) / 2 of the fragment, columns c + 8, c + 9 its other word
         const int c = j & 15;
-        mw[(c & 7) + (c >> 3)] = hf2(m[0], m[1]);
-        mw[(c & 7) + (c >> 3) + 2] = hf2(m[2], m[3]);
+        split2(m[0], m[1], mw[(c & 7) + (c >> 3)], ml[(c & 7) + (c >> 3)]);
+        split2(m[2], m[3], mw[(c & 7) + (c >> 3) + 2], ml[(c & 7) + (c >> 3) + 2]);
       }
       if (lane >= 16 * ks) {
         st32(frow + kBlkM + frag_index(lane >> 3, ks) * kFragBytes, mw);
+        st32(frow + kBlkM + (kFrags + frag_index(lane >> 3, ks)) * kFragBytes, ml);
       }
     }
     __syncwarp();
@@ -400,9 +402,9 @@ constexpr int kVBytes = kC * kVPitch;
 template <int N>
 struct ChunkSmem {
   static __host__ __device__ constexpr int stage(int heads) { return (kImgBytes<N> + heads * kBlkBytes + 127) / 128 * 128; }
-  // what a tile's warp hands to its helper for a chunk: 16-column fragments of S's first pieces, then
-  // the fragments of u~ and two scales; two chunks, then the helper's y tile
-  static constexpr int kHand = (N / 16 + kSteps) * 512 + 16;
+  // what a tile's warp hands to its helper for a chunk: 16-column fragments of S's first pieces and of
+  // its second ones, then those of u~ and two scales; two chunks, then the helper's y tile
+  static constexpr int kHandU = 2 * (N / 16) * 512, kHandS = kHandU + 2 * kSteps * 512, kHand = kHandS + 16;
   static constexpr int kHelp = 2 * kHand + kVBytes;
   static __host__ __device__ constexpr int bytes(int stages, int heads, bool help) {
     return stages * stage(heads) + kWarps * (2 * kVBytes + (help ? kHelp : 0));
@@ -524,6 +526,26 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
     }
     __syncwarp();
   };
+  // O += u M^T over 16 tokens, of two pieces each: first x first, first x second, second x first
+  auto add_mu = [&](float (*O)[4], const uint32_t (*a)[4], const unsigned char* blk, int ks) {
+    uint2 b[2][kTiles];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int j = 2 * ks; j < kTiles; ++j)
+        b[k][j] = *reinterpret_cast<const uint2*>(blk + lane * 8 + kBlkM + (k * kFrags + frag_index(j, ks)) * kFragBytes);
+#pragma unroll
+    for (int x = 0; x < 3; ++x)
+#pragma unroll
+      for (int j = 2 * ks; j < kTiles; ++j) mma16816(O[j], a[x >> 1], b[x & 1][j].x, b[x & 1][j].y);
+  };
+  auto hand_put = [&](unsigned char* at, const uint32_t* a) {
+    *reinterpret_cast<uint4*>(at + lane * 16) = make_uint4(a[0], a[1], a[2], a[3]);
+  };
+  auto hand_get = [&](const unsigned char* at, uint32_t* a) {
+    const uint4 q = *reinterpret_cast<const uint4*>(at + lane * 16);
+    a[0] = q.x; a[1] = q.y; a[2] = q.z; a[3] = q.w;
+  };
   unsigned char* hand = sm + stages * stage + kWarps * 2 * kVBytes + warp * L::kHelp;
   if constexpr (HELP) {
     if (helper) {
@@ -544,17 +566,19 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
         float O[kTiles][4] = {};
 #pragma unroll
         for (int ks = 0; ks < N / 16; ++ks) {
-          const uint4 q = *reinterpret_cast<const uint4*>(in + ks * 512 + lane * 16);
-          const uint32_t a[4] = {q.x, q.y, q.z, q.w};
+          uint32_t a[2][4], d[kTiles / 2][4];
 #pragma unroll
-          for (int j = 0; j < kTiles; j += 2) {
-            uint32_t d[4];
-            ldsm4(d, st + kC * N * 2 + tile_off<N>(8 * (j + (lane >> 4)) + (lane & 7), 2 * ks + ((lane >> 3) & 1)));
-            mma16816(O[j], a, d[0], d[1]);
-            mma16816(O[j + 1], a, d[2], d[3]);
+          for (int x = 0; x < 2; ++x) hand_get(in + (x * (N / 16) + ks) * 512, a[x]);
+#pragma unroll
+          for (int j = 0; j < kTiles; j += 2)
+            ldsm4(d[j / 2], st + kC * N * 2 + tile_off<N>(8 * (j + (lane >> 4)) + (lane & 7), 2 * ks + ((lane >> 3) & 1)));
+#pragma unroll
+          for (int x = 0; x < 2 * kTiles; ++x) {
+            const int j = x % kTiles;
+            mma16816(O[j], a[x / kTiles], d[j / 2][2 * (j & 1)], d[j / 2][2 * (j & 1) + 1]);
           }
         }
-        const float2 sc = *reinterpret_cast<const float2*>(in + (N / 16 + kSteps) * 512);
+        const float2 sc = *reinterpret_cast<const float2*>(in + L::kHandS);
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) {
           float2 eg = *reinterpret_cast<const float2*>(fac + 2 * kC + 8 * j + (lane & 3) * 2);
@@ -565,13 +589,10 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
         }
 #pragma unroll
         for (int ks = 0; ks < kSteps; ++ks) {
-          const uint4 q = *reinterpret_cast<const uint4*>(in + (N / 16 + ks) * 512 + lane * 16);
-          const uint32_t a[4] = {q.x, q.y, q.z, q.w};
+          uint32_t a[2][4];
 #pragma unroll
-          for (int j = 2 * ks; j < kTiles; ++j) {
-            const uint2 b = *reinterpret_cast<const uint2*>(blk + lane * 8 + kBlkM + frag_index(j, ks) * kFragBytes);
-            mma16816(O[j], a, b.x, b.y);
-          }
+          for (int x = 0; x < 2; ++x) hand_get(in + L::kHandU + (2 * ks + x) * 512, a[x]);
+          add_mu(O, a, blk, ks);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&taken[warp][c & 1]);
@@ -663,18 +684,18 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
       }
       // products into one accumulator are apart by a round over the tiles; the next pieces between them
 #pragma unroll
-      for (int x = 0; x < 3 * kTiles; ++x) {
+      for (int x = 0; x < 4 * kTiles; ++x) {
         const int j = x % kTiles, r = x / kTiles;
-        if (r == 1) {
-          if (!HELP) mma16816(O[j], sa[ks & 1][0], d[j / 2][2 * (j & 1)], d[j / 2][2 * (j & 1) + 1]);
+        if (r & 1) {
+          if (!HELP) mma16816(O[j], sa[ks & 1][r / 2], d[j / 2][2 * (j & 1)], d[j / 2][2 * (j & 1) + 1]);
         } else {
           mma16816(Pm[j], sa[ks & 1][r / 2], b[j / 2][2 * (j & 1)], b[j / 2][2 * (j & 1) + 1]);
         }
-        if (x % 3 == 0 && ks + 1 < N / 16) pieces(ks + 1, x / 3);
+        if (x % 4 == 0 && ks + 1 < N / 16) pieces(ks + 1, x / 4);
       }
       if (HELP)
-        *reinterpret_cast<uint4*>(out + ks * 512 + lane * 16) =
-            make_uint4(sa[ks & 1][0][0], sa[ks & 1][0][1], sa[ks & 1][0][2], sa[ks & 1][0][3]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) hand_put(out + (x * (N / 16) + ks) * 512, sa[ks & 1][x]);
     }
     // r = beta (v - e^G S k), in place
     float rmax = 0.0f;
@@ -748,24 +769,22 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
     // O += U M^T;  S += U' K
 #pragma unroll
     for (int ks = 0; ks < kSteps; ++ks) {
-      uint32_t a[4], au[2][4];
+      uint32_t a[2][4], au[2][4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 et = *reinterpret_cast<const float2*>(fac + 4 * kC + 16 * ks + 8 * (e >> 1) + (lane & 3) * 2);
         const float x = us * U[2 * ks + (e >> 1)][2 * (e & 1)], y = us * U[2 * ks + (e >> 1)][2 * (e & 1) + 1];
-        a[e] = hf2(x, y);
+        split2(x, y, a[0][e], a[1][e]);
         split2(et.x * x, et.y * y, au[0][e], au[1][e]);
       }
-      if (HELP)
-        *reinterpret_cast<uint4*>(out + (N / 16 + ks) * 512 + lane * 16) = make_uint4(a[0], a[1], a[2], a[3]);
-      else
+      if (HELP) {
 #pragma unroll
-      for (int j = 2 * ks; j < kTiles; ++j) {
-        const uint2 b = *reinterpret_cast<const uint2*>(tf + kBlkM + frag_index(j, ks) * kFragBytes);
-        mma16816(O[j], a, b.x, b.y);
+        for (int x = 0; x < 2; ++x) hand_put(out + L::kHandU + (2 * ks + x) * 512, a[x]);
+      } else {
+        add_mu(O, a, blk, ks);
       }
       if (HELP && ks == kSteps - 1) {
-        if (lane == 0) *reinterpret_cast<float2*>(out + (N / 16 + kSteps) * 512) = make_float2(os, su.inv);
+        if (lane == 0) *reinterpret_cast<float2*>(out + L::kHandS) = make_float2(os, su.inv);
         __syncwarp();
         if (lane == 0) mbar_arrive(&handed[warp][c & 1]);
       }

@@ -514,3 +514,24 @@ def test_a_copy_that_never_completes_times_out(b, T):
     assert torch.equal(got[0][1:], want[0][1:]) and torch.equal(got[1][1:], want[1][1:])
     again = gated_delta_chunk_scan(*x, return_final_states=True, status=status.zero_())
     assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1]) and int(status) == 0
+
+
+def _both_walks():
+    """A call with fewer CTAs than SMs and one with more."""
+    return pytest.mark.parametrize("b,H", [(1, 2), (80, 8)])
+
+
+@_both_walks()
+@pytest.mark.parametrize("N,init", [(64, True), (128, False), (128, True)])
+def test_an_output_is_the_formula_rounded_once(b, H, N, init):
+    """y is formed in fp32 and rounded once: it equals the rounded formula but where that lies next to a border
+    between two values.  With every term off by 2^-20 (pieces of 22 bits, fp32 sums) and terms that add up to
+    sqrt(N) of the output, an output is off by 2^-16.5 before its rounding; a share of that over a step (2^-7 at
+    most) of the values falls on the other side, so the norm of the difference is below sqrt(2^-16.5 2^-7) = 2.9e-4."""
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    d = _inputs(b, 100, H, 1, 48, N, seed=30)
+    x = [d[n] for n in ("q", "k", "v", "g", "beta")]
+    s0 = d["s0"] if init else None
+    y = gated_delta_chunk_scan(*x, initial_states=s0)
+    yr, _ = OD.gated_delta_scan(*x, S0=s0)
+    assert _rel(y, yr.bfloat16()) <= 3e-4
