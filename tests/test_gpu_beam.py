@@ -226,3 +226,71 @@ def test_long_parts(n, order, dtype):
     _check([t[:1] for t in got], x[None], s[:1], n)
     for t in got:
         assert torch.equal(t, t[:1].expand_as(t))
+
+
+def _best(logits, scores, n):
+    """(totals fp64, parents, tokens) by a sort of (score + x) - lse in 64 bits, as the totals are defined: total
+    descending, then beam, then logit descending, then token."""
+    x = logits.double().cpu()
+    top = x.amax(-1, keepdim=True)
+    total = (scores.double().cpu()[..., None] + x) - ((x - top).exp().sum(-1, keepdim=True).log() + top)
+    b, K, V = x.shape
+    got = []
+    for i in range(b):
+        rank = torch.sort(x[i], dim=-1, descending=True, stable=True).indices[:, :n]
+        kept = [(-float(total[i, k, t]), k, r, t) for k in range(K) for r, t in enumerate(rank[k].tolist())]
+        got.append(sorted(kept)[:n])
+    pick = lambda j, dt: torch.tensor([[c[j] for c in row] for row in got], dtype=dt)  # noqa: E731
+    return -pick(0, torch.float64), pick(1, torch.long), pick(3, torch.long)
+
+
+def _size(logits, parents):
+    """The largest magnitude of each continued beam's logits that count in its sum (the largest is one)."""
+    return logits.double().amax(-1).abs().cpu().gather(1, parents)
+
+
+def _check_best(got, logits, scores, n):
+    """A total is one fp32 rounding (2^-24 of it) of a sum whose log-sum-exp, with d = max - x, has terms off by
+    3 2^-24 d in the exponent (the mean of d under the softmax is at most ln V), by 2^-22 of themselves and of
+    their rescaling, and by 2^-24 for each of the at most 32 + V / 512 additions in turn.  Only the three 64-bit
+    roundings behind a total grow with the logits."""
+    ws, wp, wt = _best(logits, scores, n)
+    V = logits.shape[-1]
+    assert torch.equal(got[1].cpu().long(), wp) and torch.equal(got[2].cpu().long(), wt)
+    bound = 2.0 ** -24 * (ws.abs() + 3 * math.log(V) + 8 + 32 + V / 512) + 3 * 2.0 ** -53 * _size(logits, wp)
+    err = (got[0].cpu().double() - ws).abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
+
+
+@pytest.mark.parametrize("value", [-1e4, -1e9, -1e10, -1e12, -1e18, -1e20, -1e30, -3e38])
+@pytest.mark.parametrize("where", ["most", "tail", "head"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_finite_masks(value, where, dtype):
+    """Banned tokens at a large negative number: a thread, or all of a part, sees nothing else at first or at
+    all, and adds nothing to the sum."""
+    from nested_ssm_b200 import beam_select
+    V = 20001
+    x, s = _case(2, 3, V, dtype, seed=11)
+    keep = torch.zeros(V, dtype=torch.bool, device="cuda")
+    keep[{"most": slice(5, None, 997), "tail": slice(0, 1200), "head": slice(V - 37, None)}[where]] = True
+    x.masked_fill_(~keep, value)
+    _check_best(beam_select(x, s, 8), x, s, 8)
+
+
+@pytest.mark.parametrize("offset", [1e3, -1e3, 1e5, -1e5, 1e6, -1e6, 1e8, -1e8, -1e9, 1e20, -1e30])
+@pytest.mark.parametrize("dtype,V", [(torch.float32, 5000), (torch.bfloat16, 30000)])
+def test_logits_far_from_zero(offset, dtype, V):
+    """The same selection at any offset, as far as the type holds the differences."""
+    from nested_ssm_b200 import beam_select
+    x, s = _case(3, 4, V, dtype, seed=12)
+    x = (x.double() + offset).to(dtype)
+    _check_best(beam_select(x, s, 6), x, s, 6)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_beams_of_one_large_value(dtype):
+    """A beam whose every token has the same large value has finite totals, whatever the value."""
+    from nested_ssm_b200 import beam_select
+    x, s = _case(3, 3, 9000, dtype, seed=13)
+    x[0, 1], x[1, 0], x[2] = -1e30, 3e38, torch.finfo(dtype).min
+    _check_best(beam_select(x, s, 7), x, s, 7)
