@@ -500,7 +500,8 @@ NSSM_API int nssm_slot_copy(const nssm_slot_buffer* bufs, int32_t nbuf, int32_t 
 /* Row r continues row parents[r] (within its group of `group` rows; group == rows for indices over
  * the whole batch).  The first child of a parent keeps the parent's slot, every other child takes
  * the slot of a row without children, in row order, and the parent's state is copied there: the
- * fewest copies.  new_slots [rows].  A row whose parent is padded becomes padded. */
+ * fewest copies.  new_slots [rows].  A row whose parent is padded becomes padded.  A slot that two rows
+ * name (bit 3) is never given to another row; a child for which no slot is left becomes padded (bit 3). */
 NSSM_API int nssm_slot_reorder(const nssm_slot_buffer* bufs, int32_t nbuf, int32_t num_slots, const int32_t* slots,
                                const int32_t* parents, int32_t rows, int32_t group, int32_t pad_slot_id,
                                int32_t* new_slots, void* workspace, size_t workspace_bytes, int32_t* status,

@@ -104,6 +104,14 @@ __device__ __forceinline__ void make_plan(const PlanParams& p, uint32_t* sm, int
       const int r = r0 + j;
       parent[j] = -1;
       if (r >= p.n) continue;
+      const int mine = p.a[r];      // slots that two rows name: wr2
+      if (mine != p.pad && mine >= 0 && mine < p.S) {
+        const uint32_t m = 1u << (mine & 31);
+        if (atomicOr(&wr[mine >> 5], m) & m) {
+          atomicOr(&wr2[mine >> 5], m);
+          bad |= STATUS_CONFLICT;
+        }
+      }
       const int q = p.b[r], base = r / p.group * p.group;
       if (q < 0 || q >= min(p.group, p.n - base)) { bad |= STATUS_BAD_SLOT_BIT; continue; }
       const int s = p.a[base + q];
@@ -113,14 +121,14 @@ __device__ __forceinline__ void make_plan(const PlanParams& p, uint32_t* sm, int
       atomicMin(&first[base + q], r);
     }
     __syncthreads();
-    int2 cnt = make_int2(0, 0);   // x: children after the first, y: live rows without a child
+    int2 cnt = make_int2(0, 0);   // x: children after the first, y: live rows without a child, in slots of their own
     bool extra[kRowsPer], free_row[kRowsPer];
 #pragma unroll
     for (int j = 0; j < kRowsPer; ++j) {
       const int r = r0 + j;
       extra[j] = parent[j] >= 0 && first[parent[j]] != r;
       const int s = r < p.n ? p.a[r] : p.pad;
-      free_row[j] = r < p.n && s != p.pad && s >= 0 && s < p.S && first[r] == 0x7fffffff;
+      free_row[j] = r < p.n && s != p.pad && s >= 0 && s < p.S && first[r] == 0x7fffffff && !bit_set(wr2, s);
       cnt.x += extra[j]; cnt.y += free_row[j];
     }
     int2 at = block_scan2<NT>(cnt, &total, warp_sums);
@@ -129,6 +137,7 @@ __device__ __forceinline__ void make_plan(const PlanParams& p, uint32_t* sm, int
     for (int j = 0; j < kRowsPer; ++j)
       if (free_row[j]) freed[at.y++] = p.a[r0 + j];
     __syncthreads();
+    for (int i = threadIdx.x; i < words; i += NT) wr[i] = wr2[i] = 0;
 #pragma unroll
     for (int j = 0; j < kRowsPer; ++j) {
       src[j] = dst[j] = -1;
@@ -139,7 +148,7 @@ __device__ __forceinline__ void make_plan(const PlanParams& p, uint32_t* sm, int
         if (at.x < nfree) {
           src[j] = s;
           s = dst[j] = freed[at.x];
-        } else {            // more children than slots: a padded row was to be continued
+        } else {            // more children than slots: a row that is padded or shares its slot was to be continued
           bad |= STATUS_CONFLICT;
           s = p.pad;
         }

@@ -140,7 +140,9 @@ def reorder_slots(buffers, slots: torch.Tensor, parents: torch.Tensor, pad_slot_
     ``slots`` and ``parents`` ``[b, K]``: parents are beams of the same prompt
     (:func:`~nested_ssm_b200.beam.beam_select`); 1-D: parents are rows of the whole batch.  The first
     child of a row keeps its slot, every other child takes the slot of a row without children and
-    gets a copy of the state there: the fewest copies.  A row whose parent is padded becomes padded."""
+    gets a copy of the state there: the fewest copies.  A row whose parent is padded becomes padded.  A slot that
+    two rows name is reported and never given to another row; a child for which no slot is left is reported and
+    becomes padded."""
     shape = slots.shape
     if parents.shape != shape:
         raise ValueError(f"parents {tuple(parents.shape)} must have slots' shape {tuple(shape)}")

@@ -310,3 +310,32 @@ def test_two_calls_at_once_on_two_streams():
     for y, sel in got:
         assert torch.equal(y, ref[0]) and all(torch.equal(m, n) for m, n in zip(sel, ref[1]))
     bufs.check_status()
+
+
+@pytest.mark.parametrize("slots,parents,new,moves", [
+    ([4, 4, 6], [0, 2, 2], [4, 6, -1], []),                       # row 0 lives on in the slot that row 1 also names
+    ([4, 6, 4], [1, 1, 2], [6, -1, 4], []),
+    ([4, 4, 4], [0, 0, 0], [4, -1, -1], []),                      # rows that still share one slot
+    ([4, 4, 6, 9], [0, 2, 2, 2], [4, 6, 9, -1], [(6, 9)]),        # the free slot that one row alone names is given
+    ([4, 4, 6, 9], [2, 2, 3, 3], [6, -1, 9, -1], []),             # nobody continues 4, but two rows name it
+])
+def test_reorder_gives_no_slot_that_another_row_names(slots, parents, new, moves):
+    """A slot named twice is reported and never counts as free: nobody's state is written over."""
+    from nested_ssm_b200 import StateBuffers, reorder_slots
+    t = [torch.arange(2 * 12 * 4, dtype=torch.float32, device="cuda").view(2, 12, 4)]
+    bufs = StateBuffers(t, slot_dim=1)
+    want = _apply(t, moves)
+    got = reorder_slots(bufs, _i32(slots), _i32(parents))
+    assert got.tolist() == new
+    _same(t, want)
+    assert int(bufs.status) == 8
+
+
+def test_reorder_reports_a_slot_named_twice_without_moves():
+    from nested_ssm_b200 import StateBuffers, reorder_slots
+    t = [torch.arange(12 * 4, dtype=torch.float32, device="cuda").view(12, 4)]
+    bufs = StateBuffers(t)
+    want = [t[0].clone()]
+    assert reorder_slots(bufs, _i32([[4, 7], [7, -1]]), _i32([[0, 1], [0, 1]])).tolist() == [[4, 7], [7, -1]]
+    _same(t, want)
+    assert int(bufs.status) == 8
