@@ -429,7 +429,8 @@ NSSM_API size_t nssm_sizeof_delta_step_args(void);
 /* Prompts: y of every token and the state after the last one.  With cu_seqlens the batch is
  * packed: sequence s has the tokens cu_seqlens[s] .. cu_seqlens[s+1] of one row of `seqlen`
  * tokens (the _b strides of the inputs are not used); tokens outside every sequence are not
- * read, and their y is not written.  Sequences must not overlap.  g may be -inf; any other value of
+ * read, and their y is not written.  Sequences with bad bounds are skipped and touch no other.  Sequences must not
+ * overlap: the y of shared tokens is either one's, and those without room in the workspace are skipped.  g may be -inf; any other value of
  * a sequence that is not finite reaches every y of its block of 32 tokens, and the state.  q, k, v, y bf16; token strides multiples of 8 elements,
  * bases 16-byte aligned; (group, dstate) and (head, headdim) packed; heads of g and beta packed. */
 typedef struct {
@@ -459,7 +460,7 @@ typedef struct {
   void* workspace;        /* nssm_delta_scan_workspace_bytes(), 32-byte aligned      */
   size_t workspace_bytes;
   int32_t* status;        /* optional device word, bit 1 = a wait on a copy timed out, bit 3 = bad
-                             cu_seqlens (that sequence is skipped)                   */
+                             cu_seqlens (the sequence is skipped)                    */
 } nssm_delta_scan_args;
 
 NSSM_API size_t nssm_delta_scan_workspace_bytes(int32_t batch, int32_t seqlen, int32_t nheads, int32_t ngroups,

@@ -44,8 +44,8 @@ void slices(int P, int64_t heads, int* ns, int* rows) {
 
 using nssm::kC;
 
-// Workspace chunks: of each sequence its own; a packed sequence of `len` tokens from token a on
-// takes ceil(len / C) from a / C + s on, which stay below seqlen / C + batch.
+// Workspace chunks: of each sequence its own.  Packed sequences that do not overlap take
+// sum ceil(len / C) <= seqlen / C + batch.
 int64_t ws_chunks(int batch, int seqlen, int packed) {
   return packed ? (int64_t)seqlen / kC + batch : (int64_t)batch * ((seqlen + kC - 1) / kC);
 }

@@ -160,10 +160,12 @@ __device__ __forceinline__ float ex2(float x) {   // 2^x, 2 ulp
   return y;
 }
 
-// Workspace chunk of a sequence's first one: a packed sequence s has the chunks from
-// cu[s] / C + s on, which never overlap for ascending bounds.
-__device__ __forceinline__ int chunk_base(const DeltaChunkParams& p, int s) {
-  return p.s.cu ? p.s.cu[s] / kC + s : s * p.per_seq;
+// Chunks of sequence i, 0 where its bounds are bad.  Packed sequences take the workspace's chunks in their
+// order, each behind those before it, so that no bounds let two sequences share one; a sequence for which there is
+// no room (only sequences that overlap need more than there is) counts as bad.
+__device__ __forceinline__ int seq_chunks(const DeltaScanParams& p, int i) {
+  int batch, t0, len;
+  return delta_seq(p, i, &batch, &t0, &len) ? (len + kC - 1) / kC : 0;
 }
 
 // ---------------------------------------------------------------- T and M of every chunk
@@ -192,27 +194,48 @@ template <int N>
 __global__ void __launch_bounds__(kPrepThreads, 7) delta_prep_kernel(const DeltaChunkParams p) {
   using L = PrepSmem<N>;
   extern __shared__ __align__(128) unsigned char sm[];
-  __shared__ int s_seq;
+  __shared__ int s_seq, s_first;
+  __shared__ int64_t s_sum[kPrepWarps];
   const int slot = blockIdx.x, grp = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int s = -1;
+  int s = 0, first = 0;    // the sequence and its first chunk in the workspace
   if (!p.s.cu) {
     s = slot / p.per_seq;
+    first = s * p.per_seq;
   } else {
+    // each thread counts the chunks of a run of sequences; the one whose run has this chunk finds the sequence
+    const int per = (p.s.B + kPrepThreads - 1) / kPrepThreads, i0 = min(tid * per, p.s.B), i1 = min(i0 + per, p.s.B);
+    int64_t mine = 0;
+    for (int i = i0; i < i1; ++i) mine += seq_chunks(p.s, i);
+    int64_t to = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, to, o);
+      if (lane >= o) to += y;
+    }
+    if (lane == 31) s_sum[warp] = to;
     if (tid == 0) s_seq = -1;
     __syncthreads();
-    for (int i = tid; i < p.s.B; i += kPrepThreads) {
-      int b0, t0, len;
-      if (!delta_seq(p.s, i, &b0, &t0, &len)) continue;
-      const int c = slot - chunk_base(p, i);
-      if (c >= 0 && c < (len + kC - 1) / kC) s_seq = i;
+    for (int w = 0; w < warp; ++w) to += s_sum[w];
+    if (to > slot && to - mine <= slot) {
+      int at = (int)(to - mine);
+      for (int i = i0;; ++i) {
+        const int n = seq_chunks(p.s, i);
+        if (slot < at + n) {
+          s_seq = i;
+          s_first = at;
+          break;
+        }
+        at += n;
+      }
     }
     __syncthreads();
     s = s_seq;
     if (s < 0) return;
+    first = s_first;
   }
   int batch, t0, len;
   delta_seq(p.s, s, &batch, &t0, &len);
-  const int c0 = (slot - chunk_base(p, s)) * kC;
+  const int c0 = (slot - first) * kC;
   const int nt = min(kC, len - c0);       // tokens of this chunk; the others count as zeros
   const int64_t tok = (int64_t)t0 + c0;
   const uint32_t sk = sm32(sm), sq = sk + kC * N * 2;
@@ -453,6 +476,15 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
   const int nh = (tg * kWarps + warps - 1) / p.tiles - h0 + 1;
   const int hr = (tg * kWarps + warp) / p.tiles;                // the warp's
   const int h = grp * rep + hr, row_h = ((tg * kWarps + warp) - hr * p.tiles) * 16;
+  const int nchunk = (len + kC - 1) / kC;
+  __shared__ int64_t sums[2 * kWarps];      // chunks of the packed sequences before this one, by warps
+  if (p.s.cu) {
+    int64_t n = 0;
+    for (int i = tid; i < s; i += blockDim.x) n += seq_chunks(p.s, i);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    if (lane == 0) sums[role] = n;
+  }
   if (tid == 0) {
     for (int i = 0; i < kChunkStages; ++i) {
       mbar_init(&full[i], 1);
@@ -466,14 +498,21 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
     fence_mbar_init();
   }
   __syncthreads();
+  int64_t slot0 = (int64_t)s * p.per_seq;       // its first chunk in the workspace
+  if (p.s.cu) {
+    slot0 = 0;
+    for (int w = 0; w < (HELP ? 2 : 1) * kWarps; ++w) slot0 += sums[w];
+    if (nchunk && slot0 + nchunk > p.chunks) {
+      if (p.s.status && blockIdx.x == 0 && tid == 0) atomicOr(p.s.status, STATUS_CONFLICT);
+      return;
+    }
+  }
   if (warp >= warps) return;
-  const int nchunk = (len + kC - 1) / kC;
-  const int slot0 = chunk_base(p, s);
   const uint32_t base = sm32(sm);
   const int stage = L::stage(p.heads), stages = p.stages, ahead = p.stages - 2;
   const __nv_bfloat16* gv = p.s.v + batch * p.s.v_b + (int64_t)t0 * p.s.v_t + h * p.s.P + row_h;
-  const unsigned char* gimg = p.img + ((int64_t)slot0 * p.s.G + grp) * kImgBytes<N>;
-  const unsigned char* gblk = p.blk + ((int64_t)slot0 * p.s.H + grp * rep + h0) * kBlkBytes;
+  const unsigned char* gimg = p.img + (slot0 * p.s.G + grp) * kImgBytes<N>;
+  const unsigned char* gblk = p.blk + (slot0 * p.s.H + grp * rep + h0) * kBlkBytes;
 
   // K, Q, T and M of chunk c into its stage, by one warp
   auto load = [&](int c) {

@@ -535,3 +535,70 @@ def test_an_output_is_the_formula_rounded_once(b, H, N, init):
     y = gated_delta_chunk_scan(*x, initial_states=s0)
     yr, _ = OD.gated_delta_scan(*x, S0=s0)
     assert _rel(y, yr.bfloat16()) <= 3e-4
+
+
+@pytest.mark.parametrize("repeat", [1, 40])
+def test_scan_bad_bounds_touch_no_other_sequence(repeat):
+    """Sequences whose bounds descend lie between others that end and begin anywhere, 40 times over the tokens of
+    the first ones too: those with good bounds of their own tokens are as ever."""
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    step = 100
+    d = _inputs(1, step * repeat, 2, 1, 32, 64, seed=31)
+    x = [d[n] for n in ("q", "k", "v", "g", "beta")]
+    cu, good = [], []
+    for r in reversed(range(repeat)):         # the last tokens first: every second sequence descends
+        good += [(len(cu), step * r + 50, step * r + 100), (len(cu) + 2, step * r, step * r + 30)]
+        cu += [step * r + 50, step * r + 100, step * r, step * r + 30]
+    # (30 of one group to 50 of the one before it descends too)
+    n = len(cu) - 1
+    out = torch.full((1, step * repeat, 2, 32), 3.0, dtype=torch.bfloat16, device="cuda")
+    fin = torch.full((n, 2, 32, 64), 5.0, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    gated_delta_chunk_scan(*x, cu_seqlens=torch.tensor(cu, dtype=torch.int32, device="cuda"), out=out, final_states=fin,
+                           status=status)
+    assert int(status) == 8
+    names = {s for s, _, _ in good}
+    for s, a, e in good:
+        yr, Sr = OD.gated_delta_scan(*(t[:, a:e] for t in x))
+        _check_y(out[:, a:e], yr, f"sequence {s}")
+        _check_state(fin[s], Sr[0], f"sequence {s}")
+    bad = [s for s in range(n) if s not in names]
+    assert all(cu[s + 1] < cu[s] for s in bad) and bool((fin[bad] == 5.0).all())
+    for r in range(repeat):
+        assert bool((out[:, step * r + 30:step * r + 50] == 3.0).all())
+
+
+def test_scan_overlapping_sequences_without_room_are_skipped():
+    """More blocks than the tokens can have: the sequences that still fit are run, the others reported."""
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    d = _inputs(1, 100, 2, 1, 32, 64, seed=32)
+    x = [d[n] for n in ("q", "k", "v", "g", "beta")]
+    cu = torch.tensor([0, 100] * 3, dtype=torch.int32, device="cuda")      # 3 x 4 blocks; 100 / 32 + 5 = 8 fit
+    fin = torch.full((5, 2, 32, 64), 5.0, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    y = gated_delta_chunk_scan(*x, cu_seqlens=cu, final_states=fin, status=status)
+    yr, Sr = OD.gated_delta_scan(*x)
+    _check_y(y, yr)
+    _check_state(fin[0], Sr[0])
+    _check_state(fin[2], Sr[0])
+    assert int(status) == 8 and all(bool((fin[s] == 5.0).all()) for s in (1, 3, 4))
+
+
+def test_scan_of_many_packed_sequences():
+    """More sequences than a CTA ranks or has threads, empty ones among them."""
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    lens = [(7 * i) % 37 if i % 5 else 0 for i in range(700)]
+    d = _inputs(1, sum(lens) + 5, 2, 1, 16, 64, seed=33)
+    x = [d[n] for n in ("q", "k", "v", "g", "beta")]
+    at = [0]
+    for n in lens:
+        at.append(at[-1] + n)
+    y, S = gated_delta_chunk_scan(*x, cu_seqlens=torch.tensor(at, dtype=torch.int32, device="cuda"), return_final_states=True)
+    for s in list(range(0, 700, 41)) + [698, 699]:
+        part = [t[:, at[s]:at[s + 1]] for t in x]
+        if lens[s]:
+            yr, Sr = OD.gated_delta_scan(*part)
+            _check_y(y[:, at[s]:at[s + 1]], yr, f"sequence {s}")
+            _check_state(S[s], Sr[0], f"sequence {s}")
+        else:
+            assert float(S[s].abs().max()) == 0.0
