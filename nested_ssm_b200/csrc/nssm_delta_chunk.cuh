@@ -781,21 +781,25 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
     // The scale of the state that follows: no element of it exceeds
     //   e^{G_C} max |S| + 32 max |k^| max |u~| max(e^{G_C - G}, 1),   |k^| < 512,
     // so its pieces can be taken from the registers as they are.  The bound may be 2^17 above the
-    // state before its second pieces run into fp16's smallest values.
+    // state before its second pieces run into fp16's smallest values.  (Where every first piece is zero, |S| may be
+    // just below 2^-24.)
+    // O has a scale of its own, so.s, with so.s |u~| below 2^15: a chunk may read a state and forget it that is far
+    // above what it leaves.  Where S is more than 2^64 above u~, u~ loses bits instead of O leaving fp32.
     const float inv_u = fr.inv * fac[5 * kC];
     float umax = 0.0f;
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) umax = amax4(U[j], umax);
     const float egc = fac[3 * kC - 1] * 0x1p12f;
-    const float sm1 = fmaxf(__low2float(smax), __high2float(smax));
-    const Pow2 sn = warp_scale(fmaxf(2.001f * egc * su.inv * sm1, 0x1p15f * inv_u * fac[5 * kC + 1] * umax));
-    const float os = su.inv * sn.s, us = inv_u * sn.s, es = egc * os;
+    const float bs = su.inv * fmaxf(fmaxf(__low2float(smax), __high2float(smax)), 0x1p-24f);
+    const Pow2 sn = warp_scale(fmaxf(2.001f * egc * bs, 0x1p15f * inv_u * fac[5 * kC + 1] * umax));
+    const Pow2 so = warp_scale(fmaxf(0x1p-64f * bs, inv_u * umax));
+    const float os = su.inv * so.s, uo = inv_u * so.s, us = inv_u * sn.s, es = egc * su.inv * sn.s;
     su = sn;
 #pragma unroll
     for (int t = 0; t < N / 8; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) S[t][e] *= es;
-    // O = 2^-12 e^G S q^ + M u~
+    // O = so.s (2^-12 e^G S q^ + M u~)
     if (!HELP)
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) {
@@ -812,9 +816,9 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 et = *reinterpret_cast<const float2*>(fac + 4 * kC + 16 * ks + 8 * (e >> 1) + (lane & 3) * 2);
-        const float x = us * U[2 * ks + (e >> 1)][2 * (e & 1)], y = us * U[2 * ks + (e >> 1)][2 * (e & 1) + 1];
-        split2(x, y, a[0][e], a[1][e]);
-        split2(et.x * x, et.y * y, au[0][e], au[1][e]);
+        const float x = U[2 * ks + (e >> 1)][2 * (e & 1)], y = U[2 * ks + (e >> 1)][2 * (e & 1) + 1];
+        split2(uo * x, uo * y, a[0][e], a[1][e]);
+        split2(et.x * (us * x), et.y * (us * y), au[0][e], au[1][e]);
       }
       if (HELP) {
 #pragma unroll
@@ -823,7 +827,7 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
         add_mu(O, a, blk, ks);
       }
       if (HELP && ks == kSteps - 1) {
-        if (lane == 0) *reinterpret_cast<float2*>(out + L::kHandS) = make_float2(os, su.inv);
+        if (lane == 0) *reinterpret_cast<float2*>(out + L::kHandS) = make_float2(os, so.inv);
         __syncwarp();
         if (lane == 0) mbar_arrive(&handed[warp][c & 1]);
       }
@@ -839,7 +843,7 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
           for (int x = 0; x < 4; ++x) mma16816(S[t + x], au[i], b[x / 2][2 * (x & 1)], b[x / 2][2 * (x & 1) + 1]);
       }
     }
-    if (!HELP) finish(O, fac, su.inv, vt, c);
+    if (!HELP) finish(O, fac, so.inv, vt, c);
     __syncwarp();
     if (lane == 0) mbar_arrive(&empty[si]);
   }

@@ -602,3 +602,50 @@ def test_scan_of_many_packed_sequences():
             _check_state(S[s], Sr[0], f"sequence {s}")
         else:
             assert float(S[s].abs().max()) == 0.0
+
+
+@_both_walks()
+@pytest.mark.parametrize("size", [1.0, 1e3, 1e5, 1e9, 1e25])
+@pytest.mark.parametrize("how", ["at once", "at the first token", "by degrees"])
+def test_scan_forgets_a_large_state_without_writing(b, H, size, how):
+    """A block of 32 tokens that writes nothing (beta 0) and forgets a large state: the outputs before it are the
+    large state's, those behind it and the state start from zero."""
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    d = _inputs(b, 130, H, 1, 32, 128, seed=26)
+    d["s0"] *= size
+    d["beta"][:, :64] = 0.0
+    if how == "by degrees":
+        d["g"][:, :32] = 0.0
+        d["g"][:, 32:64] = -12.0          # e^-384: nothing of the largest state is left in fp32
+    else:
+        d["g"][:, :64] = 0.0
+        d["g"][:, 32 if how == "at the first token" else 61] = float("-inf")
+    d["v"][:, 64:70] = 0.0
+    x = [d[n] for n in ("q", "k", "v", "g", "beta")]
+    y, S = gated_delta_chunk_scan(*x, initial_states=d["s0"], return_final_states=True)
+    yr, Sr = OD.gated_delta_scan(*x, S0=d["s0"])
+    _check_y(y[:, :32], yr[:, :32], "before")
+    if how == "at once":
+        _check_y(y[:, 32:61], yr[:, 32:61], "in the block, before")
+        assert float(y[:, 61:70].abs().max()) == 0.0
+    _check_y(y[:, 70:], yr[:, 70:], "behind")
+    _check_state(S, Sr)
+    _, none = gated_delta_chunk_scan(*(t[:, :64] for t in x), initial_states=d["s0"], return_final_states=True)
+    assert float(none.abs().max()) <= 1e-30
+
+
+@_both_walks()
+def test_scan_writes_then_forgets_in_one_block(b, H):
+    """Large values written and forgotten within one block, a block without writes, then usual ones."""
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    d = _inputs(b, 130, H, 1, 32, 64, seed=27)
+    d["v"][:, :20] *= 1e5
+    d["g"][:, 31] = float("-inf")
+    d["beta"][:, 31:64] = 0.0
+    x = [d[n] for n in ("q", "k", "v", "g", "beta")]
+    y, S = gated_delta_chunk_scan(*x, return_final_states=True)
+    yr, Sr = OD.gated_delta_scan(*x)
+    _check_y(y[:, :31], yr[:, :31])
+    assert float(y[:, 31:64].abs().max()) == 0.0
+    _check_y(y[:, 64:], yr[:, 64:])
+    _check_state(S, Sr)
