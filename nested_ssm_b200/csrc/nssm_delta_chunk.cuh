@@ -30,7 +30,8 @@
 // fp16 values (11 bits each, the second holds what the first leaves), scaled by a power of two that
 // keeps the warp's values below 2^15; what is left out is below 2^-22 of a value or 2^-25.  K and Q
 // (bf16) become fp16 exactly, each token scaled by its own power of two (elements below 2^-25 of the
-// token's largest lose bits).  T, M and u go in as two pieces, so only products of two second pieces are
+// token's largest lose bits).  The r of a chunk share one scale, as do its u: those more than 2^17 below a warp's
+// largest lose bits.  T, M and u go in as two pieces, so only products of two second pieces are
 // left out, 2^-22 of a product.  y is the fp32 sum rounded once to bf16 (single fp16 operands, 2^-12, in its
 // own products moved 3e-4 of it, and one value in thirty by a step; they take 504 against 557 us for 2 x 8192
 // tokens of 32 heads, 950 against 1086 for 8 x 2048 of 128).
@@ -52,8 +53,7 @@ constexpr int kFrags = 6, kFragBytes = 256;
 __host__ __device__ constexpr int frag_index(int nt, int ks) { return nt < 2 ? nt : 2 * nt - 2 + ks; }
 // With k = sk k^ and q = sq q^ (sk, sq powers of two per token), the walk works on u~ = sk u.
 // Workspace block of a (chunk, head): two pieces of sT sk T, two of 2^-12 D (q^.k^), then per token
-// beta, beta e^G sk, 2^-12 e^G, 2^12 scale sq, e^{G_C - G}, then 1 / sT and the largest of the
-// e^{G_C - G} and 1.
+// beta, beta e^G sk, 2^-12 e^G, 2^12 scale sq, e^{G_C - G}, then 1 / sT.
 constexpr int kBlkM = 2 * kFrags * kFragBytes;
 constexpr int kBlkF = kBlkM + 2 * kFrags * kFragBytes;
 constexpr int kBlkBytes = kBlkF + 5 * kC * 4 + 32;    // whole sectors
@@ -338,10 +338,7 @@ __global__ void __launch_bounds__(kPrepThreads, 7) delta_prep_kernel(const Delta
     f[kC + lane] = bs * eg;
     f[2 * kC + lane] = eg * 0x1p-12f;
     f[3 * kC + lane] = p.s.scale * ssk[kC + lane] * 0x1p12f;
-    const float et = ex2((gh[kC - 1] - gih) + (gl[kC - 1] - gil));
-    f[4 * kC + lane] = et;
-    const uint32_t etm = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(et, 1.0f)));
-    if (lane == 1) f[5 * kC + 1] = __uint_as_float(etm);
+    f[4 * kC + lane] = ex2((gh[kC - 1] - gih) + (gl[kC - 1] - gil));
     // row `lane` of M, of A
     unsigned char* frow = blk + (lane & 7) * 32;      // its 32 bytes of each fragment
 #pragma unroll
@@ -779,19 +776,25 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
         for (int j = 2 * ks; j < kTiles; ++j) mma16816(U[j], a[x >> 1], b[x & 1][j].x, b[x & 1][j].y);
     }
     // The scale of the state that follows: no element of it exceeds
-    //   e^{G_C} max |S| + 32 max |k^| max |u~| max(e^{G_C - G}, 1),   |k^| < 512,
+    //   e^{G_C} max |S| + 32 max |k^| max |e^{G_C - G} u~|,   |k^| < 512,
     // so its pieces can be taken from the registers as they are.  The bound may be 2^17 above the
-    // state before its second pieces run into fp16's smallest values.  (Where every first piece is zero, |S| may be
-    // just below 2^-24.)
+    // state before its second pieces run into fp16's smallest values, and is seldom 2^10 above it.  (Where
+    // every first piece is zero, |S| may be just below 2^-24.)
     // O has a scale of its own, so.s, with so.s |u~| below 2^15: a chunk may read a state and forget it that is far
     // above what it leaves.  Where S is more than 2^64 above u~, u~ loses bits instead of O leaving fp32.
     const float inv_u = fr.inv * fac[5 * kC];
-    float umax = 0.0f;
+    float umax = 0.0f, wmax = 0.0f;
+    float2 et[kTiles];
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) umax = amax4(U[j], umax);
+    for (int j = 0; j < kTiles; ++j) {
+      et[j] = *reinterpret_cast<const float2*>(fac + 4 * kC + 8 * j + (lane & 3) * 2);
+      const float x = fmaxf(fabsf(U[j][0]), fabsf(U[j][2])), y = fmaxf(fabsf(U[j][1]), fabsf(U[j][3]));
+      umax = fmaxf(umax, fmaxf(x, y));
+      wmax = fmaxf(wmax, fmaxf(et[j].x * x, et[j].y * y));
+    }
     const float egc = fac[3 * kC - 1] * 0x1p12f;
     const float bs = su.inv * fmaxf(fmaxf(__low2float(smax), __high2float(smax)), 0x1p-24f);
-    const Pow2 sn = warp_scale(fmaxf(2.001f * egc * bs, 0x1p15f * inv_u * fac[5 * kC + 1] * umax));
+    const Pow2 sn = warp_scale(fmaxf(2.001f * egc * bs, 0x1p15f * inv_u * wmax));
     const Pow2 so = warp_scale(fmaxf(0x1p-64f * bs, inv_u * umax));
     const float os = su.inv * so.s, uo = inv_u * so.s, us = inv_u * sn.s, es = egc * su.inv * sn.s;
     su = sn;
@@ -815,10 +818,10 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
       uint32_t a[2][4], au[2][4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float2 et = *reinterpret_cast<const float2*>(fac + 4 * kC + 16 * ks + 8 * (e >> 1) + (lane & 3) * 2);
+        const float2 ej = et[2 * ks + (e >> 1)];
         const float x = U[2 * ks + (e >> 1)][2 * (e & 1)], y = U[2 * ks + (e >> 1)][2 * (e & 1) + 1];
         split2(uo * x, uo * y, a[0][e], a[1][e]);
-        split2(et.x * (us * x), et.y * (us * y), au[0][e], au[1][e]);
+        split2(us * (ej.x * x), us * (ej.y * y), au[0][e], au[1][e]);
       }
       if (HELP) {
 #pragma unroll

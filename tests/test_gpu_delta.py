@@ -649,3 +649,22 @@ def test_scan_writes_then_forgets_in_one_block(b, H):
     assert float(y[:, 31:64].abs().max()) == 0.0
     _check_y(y[:, 64:], yr[:, 64:])
     _check_state(S, Sr)
+
+
+@_both_walks()
+@pytest.mark.parametrize("N", [64, 128])
+@pytest.mark.parametrize("decay", [-5.0, -12.0, -20.0, -40.0])
+def test_scan_reads_a_state_that_has_decayed_since_its_writes(b, H, N, decay):
+    """Values of 1 written, then a decay of up to e^-40 in the same block: the next block reads the small state
+    to the same relative precision, and erases along its keys (v = 0)."""
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    d = _inputs(b, 96, H, 1, 48, N, seed=28)
+    d["g"][:, 16] = decay
+    d["beta"][:, 16:40] = 0.0
+    d["v"][:, 16:] = 0.0
+    x = [d[n] for n in ("q", "k", "v", "g", "beta")]
+    y, S = gated_delta_chunk_scan(*x, return_final_states=True)
+    yr, Sr = OD.gated_delta_scan(*x)
+    _check_state(S, Sr)
+    assert _rel(y[:, 32:64], yr[:, 32:64]) <= Y_TOL
+    assert _rel(y[:, 64:], yr[:, 64:]) <= Y_TOL
