@@ -52,8 +52,12 @@ constexpr int kSteps = kC / 16;
 constexpr int kFrags = 6, kFragBytes = 256;
 __host__ __device__ constexpr int frag_index(int nt, int ks) { return nt < 2 ? nt : 2 * nt - 2 + ks; }
 // With k = sk k^ and q = sq q^ (sk, sq powers of two per token), the walk works on u~ = sk u.
-// Workspace block of a (chunk, head): two pieces of sT sk T, two of 2^-12 D (q^.k^), then per token
-// beta, beta e^G sk, 2^-12 e^G, 2^12 scale sq, e^{G_C - G}, then 1 / sT.
+// Where g > 0 lets a chunk's state grow, r, u and y of its tokens grow with it; each token then has a power of two c
+// (1 while nothing has grown) that takes the growth since the smallest G out: with e^G' = c e^G and D' = e^{G'_i - G'_j}
+// <= 1 in the place of e^G and D, the walk works on r~ = c r, u~ = sk c u and c y.
+// Workspace block of a (chunk, head): two pieces of sT sk T, two of 2^-12 D' (q^.k^), then per token
+// c beta, beta e^G' sk, 2^-12 e^G', 2^12 scale sq / c, e^{G_C - G'}, then 1 / sT, e^{G_C} and the larger of e^g of
+// the first token and 1 (e^G' is not above it).
 constexpr int kBlkM = 2 * kFrags * kFragBytes;
 constexpr int kBlkF = kBlkM + 2 * kFrags * kFragBytes;
 constexpr int kBlkBytes = kBlkF + 5 * kC * 4 + 32;    // whole sectors
@@ -327,18 +331,29 @@ __global__ void __launch_bounds__(kPrepThreads, 7) delta_prep_kernel(const Delta
       const double y = __shfl_up_sync(0xffffffffu, G, o);
       if (lane >= o) G += y;
     }
+    float low = (float)G;       // the smallest so far
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float y = __shfl_up_sync(0xffffffffu, low, o);
+      if (lane >= o) low = fminf(low, y);
+    }
+    const int up = (int)fminf(ceilf((float)G - low), 126.0f);
+    G -= (double)up;            // G'
     const float gih = (float)G, gil = (float)(G - (double)gih);
     gh[lane] = gih;
     gl[lane] = gil;
     __syncwarp();
     unsigned char* blk = p.blk + ((int64_t)slot * p.s.H + h) * kBlkBytes;
     float* f = reinterpret_cast<float*>(blk + kBlkF);
+    const float c_inv = __uint_as_float((127 + up) << 23), up_end = (float)__shfl_sync(0xffffffffu, up, kC - 1);
     const float eg = ex2(gih + gil), ski = ssk[lane], bs = beta * ski;
-    f[lane] = beta;
+    f[lane] = beta * __uint_as_float((127 - up) << 23);
     f[kC + lane] = bs * eg;
     f[2 * kC + lane] = eg * 0x1p-12f;
-    f[3 * kC + lane] = p.s.scale * ssk[kC + lane] * 0x1p12f;
-    f[4 * kC + lane] = ex2((gh[kC - 1] - gih) + (gl[kC - 1] - gil));
+    f[3 * kC + lane] = p.s.scale * ssk[kC + lane] * 0x1p12f * c_inv;
+    if (lane == kC - 1) f[5 * kC + 1] = ex2(gih + gil + up_end);
+    if (lane == 0) f[5 * kC + 2] = fmaxf(eg, 1.0f);
+    f[4 * kC + lane] = ex2((gh[kC - 1] - gih) + (gl[kC - 1] - gil) + up_end);
     // row `lane` of M, of A
     unsigned char* frow = blk + (lane & 7) * 32;      // its 32 bytes of each fragment
 #pragma unroll
@@ -733,7 +748,7 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
 #pragma unroll
         for (int x = 0; x < 2; ++x) hand_put(out + (x * (N / 16) + ks) * 512, sa[ks & 1][x]);
     }
-    // r = beta (v - e^G S k), in place
+    // r~ = c beta v - beta e^G' S k, in place
     float rmax = 0.0f;
 #pragma unroll
     for (int j = 0; j < kTiles; j += 2) {
@@ -776,7 +791,7 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
         for (int j = 2 * ks; j < kTiles; ++j) mma16816(U[j], a[x >> 1], b[x & 1][j].x, b[x & 1][j].y);
     }
     // The scale of the state that follows: no element of it exceeds
-    //   e^{G_C} max |S| + 32 max |k^| max |e^{G_C - G} u~|,   |k^| < 512,
+    //   e^{G_C} max |S| + 32 max |k^| max |e^{G_C - G'} u~|,   |k^| < 512,
     // so its pieces can be taken from the registers as they are.  The bound may be 2^17 above the
     // state before its second pieces run into fp16's smallest values, and is seldom 2^10 above it.  (Where
     // every first piece is zero, |S| may be just below 2^-24.)
@@ -792,17 +807,17 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
       umax = fmaxf(umax, fmaxf(x, y));
       wmax = fmaxf(wmax, fmaxf(et[j].x * x, et[j].y * y));
     }
-    const float egc = fac[3 * kC - 1] * 0x1p12f;
+    const float egc = fac[5 * kC + 1];
     const float bs = su.inv * fmaxf(fmaxf(__low2float(smax), __high2float(smax)), 0x1p-24f);
     const Pow2 sn = warp_scale(fmaxf(2.001f * egc * bs, 0x1p15f * inv_u * wmax));
-    const Pow2 so = warp_scale(fmaxf(0x1p-64f * bs, inv_u * umax));
+    const Pow2 so = warp_scale(fmaxf(0x1p-64f * fac[5 * kC + 2] * bs, inv_u * umax));
     const float os = su.inv * so.s, uo = inv_u * so.s, us = inv_u * sn.s, es = egc * su.inv * sn.s;
     su = sn;
 #pragma unroll
     for (int t = 0; t < N / 8; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) S[t][e] *= es;
-    // O = so.s (2^-12 e^G S q^ + M u~)
+    // O = so.s (2^-12 e^G' S q^ + M u~)
     if (!HELP)
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) {

@@ -127,7 +127,7 @@ def gated_delta_chunk_scan(q, k, v, g, beta, scale: float | None = None, initial
     the rows of ``out`` outside every sequence are left as they were.  Sequences whose bounds
     do not ascend inside ``[0, T]`` are skipped and set bit 3 of the int32 ``status``; they touch no
     other.  Sequences must not overlap.  Otherwise n == b.  ``initial_states [n, H, P, N]`` fp32 (zeros without them); ``final_states`` may be the
-    same tensor.  ``g`` may be ``-inf`` (the state is forgotten); any other value of a sequence that
+    same tensor.  ``g`` may be ``-inf`` (the state is forgotten) and above 0 (it grows); any other value of a sequence that
     is not finite reaches every output of its 32-token block, those before it too, and the state."""
     qs, vs = q.shape, v.shape
     if len(qs) != 4 or k.shape != qs or len(vs) != 4:

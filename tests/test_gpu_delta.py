@@ -668,3 +668,23 @@ def test_scan_reads_a_state_that_has_decayed_since_its_writes(b, H, N, decay):
     _check_state(S, Sr)
     assert _rel(y[:, 32:64], yr[:, 32:64]) <= Y_TOL
     assert _rel(y[:, 64:], yr[:, 64:]) <= Y_TOL
+
+
+@_both_walks()
+@pytest.mark.parametrize("g,T", [(0.02, 200), (0.1, 100), (0.3, 40), (1.0, 33), (2.0, 40)])
+def test_scan_takes_states_that_grow(b, H, g, T):
+    """g above zero, with keys and queries that point the same way and use the whole of their type's range of a
+    token (every element the same size): D (q.k) is far above the state's own scale."""
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    d = _inputs(b, T, H, 1, 32, 128, seed=29)
+    one = torch.where(d["k"][:, :1] < 0, -1.0, 1.0).expand_as(d["k"]) * (255 / 256) * 128 ** -0.5
+    d["k"], d["q"] = one.bfloat16().contiguous(), one.bfloat16().contiguous()
+    d["g"] = torch.full_like(d["g"], g)
+    d["beta"] *= 0.1
+    x = [d[n] for n in ("q", "k", "v", "g", "beta")]
+    y, S = gated_delta_chunk_scan(*x, initial_states=d["s0"], return_final_states=True)
+    yr, Sr = OD.gated_delta_scan(*x, S0=d["s0"])
+    _check_state(S, Sr)
+    assert bool(torch.isfinite(y).all()) and _rel(y, yr) <= Y_TOL
+    for t in range(0, T, 16):             # and of every stretch of tokens by itself
+        assert _rel(y[:, t:t + 16], yr[:, t:t + 16]) <= Y_TOL, t
