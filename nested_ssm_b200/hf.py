@@ -27,8 +27,10 @@ cold read, ring or flush.
 """
 from __future__ import annotations
 
+import copy
+import copyreg
+import functools
 import math
-import weakref
 
 import torch
 import torch.nn.functional as F
@@ -192,29 +194,55 @@ def _lean_prefill(self, input_states, cache_params, attention_mask):
 
 
 class _FollowBeams:
-    """A cache layer's ``reorder_cache``: the rows of the cache, then the pool's slots.  A deep copy of the
-    layer gets one of its own for the same pool."""
+    """The ``reorder_cache`` of a cache layer whose state is in a pool: the layer's rows, then the pool's slots."""
 
     def __init__(self, layer, st):
-        self.layer, self.st = weakref.ref(layer), st     # (the layer holds this: no cycle)
+        self.layer, self.st = layer, st
 
     def __call__(self, beam_idx):
-        layer, st = self.layer(), self.st
-        type(layer).reorder_cache(layer, beam_idx)
+        st = self.st
+        type(self.layer).plain.reorder_cache(self.layer, beam_idx)
         slots = st["slots"]
         if st["draft"] is not None:
             reorder_slots(StateBuffers([st["draft"]]), slots, beam_idx.to(slots.device))
         st["slots"] = reorder_slots(st["pool"], slots, beam_idx.to(slots.device))
 
-    def __deepcopy__(self, memo):
-        layer = self.layer()
-        return _FollowBeams(memo.get(id(layer), layer), self.st)
+
+@functools.cache
+def _following(cls):
+    """``cls`` with a ``reorder_cache`` that takes the pool along.  A copy of such a layer has rows of its own and
+    the same pool; pickled it is a ``cls``, the pool stays with the model."""
+
+    def rows(self):
+        return {k: v for k, v in self.__dict__.items() if k != "_nssm_st"}
+
+    def shallow(self):
+        other = object.__new__(type(self))
+        other.__dict__.update(self.__dict__)
+        return other
+
+    def deep(self, memo):
+        other = memo[id(self)] = object.__new__(type(self))
+        other.__dict__.update(copy.deepcopy(rows(self), memo), _nssm_st=self._nssm_st)
+        return other
+
+    def reduce(self, protocol):
+        plain = object.__new__(cls)
+        plain.__dict__.update(rows(self))
+        return copyreg._reconstructor, (cls, object, None), plain.__getstate__()
+
+    return type(cls)(cls.__name__, (cls,), {
+        "__module__": cls.__module__, "__qualname__": cls.__qualname__, "__doc__": cls.__doc__, "plain": cls,
+        "reorder_cache": property(lambda self: _FollowBeams(self, self._nssm_st)),
+        "__copy__": shallow, "__deepcopy__": deep, "__reduce_ex__": reduce})
 
 
 def _follow_beams(layer, st) -> None:
     """Let the pool's slots follow the rows of a cache layer when beam search reorders them."""
     if hasattr(type(layer), "reorder_cache"):
-        layer.reorder_cache = _FollowBeams(layer, st)
+        if not hasattr(layer, "_nssm_st"):
+            layer.__class__ = _following(type(layer))
+        layer._nssm_st = st
 
 
 def _dispatch(self, input_states, cache_params=None, attention_mask=None):

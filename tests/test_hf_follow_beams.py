@@ -1,5 +1,6 @@
 """The hook that lets the pool's slots follow a cache layer's rows (host logic, CPU)."""
 import copy
+import pickle
 
 import torch
 
@@ -63,3 +64,26 @@ def test_a_layer_goes_with_its_last_reference(monkeypatch):
         assert gone() is None
     finally:
         gc.enable()
+
+
+def test_a_shallow_copy_reorders_its_own_rows(monkeypatch):
+    layer, st = Layer(), _state([], monkeypatch)
+    hf._follow_beams(layer, st)
+    other = copy.copy(layer)
+    other.reorder_cache(torch.tensor([3, 2, 1, 0]))
+    assert other.rows.tolist() == [3, 2, 1, 0] and layer.rows.tolist() == [0, 1, 2, 3]
+    assert st["slots"].tolist() == [2, 0, 1, 3]
+
+
+def test_a_layer_can_be_pickled_and_saved(monkeypatch, tmp_path):
+    """What is read back is a layer of the plain class: the pool stays with the model."""
+    layer, st = Layer(), _state([], monkeypatch)
+    hf._follow_beams(layer, st)
+    cache = {"layers": [layer, layer]}
+    torch.save(cache, tmp_path / "cache.pt")
+    for got in (pickle.loads(pickle.dumps(cache)), torch.load(tmp_path / "cache.pt", weights_only=False)):
+        first, second = got["layers"]
+        assert first is second and type(first) is Layer and first.rows.tolist() == [0, 1, 2, 3]
+        first.reorder_cache(torch.tensor([1, 0, 3, 2]))
+        assert first.rows.tolist() == [1, 0, 3, 2]
+    assert st["slots"].tolist() == [3, 1, 0, 2] and isinstance(layer, Layer) and layer.reorder_cache.st is st
