@@ -194,14 +194,17 @@ def _lean_prefill(self, input_states, cache_params, attention_mask):
 
 
 class _FollowBeams:
-    """The ``reorder_cache`` of a cache layer whose state is in a pool: the layer's rows, then the pool's slots."""
+    """The ``reorder_cache`` of a cache layer whose state is in a pool: the layer's rows, then the pool's slots,
+    as long as no later prefill has taken the pool for another cache."""
 
-    def __init__(self, layer, st):
-        self.layer, self.st = layer, st
+    def __init__(self, layer, st, prefill):
+        self.layer, self.st, self.prefill = layer, st, prefill
 
     def __call__(self, beam_idx):
         st = self.st
         type(self.layer).plain.reorder_cache(self.layer, beam_idx)
+        if st["prefill"] is not self.prefill:
+            return
         slots = st["slots"]
         if st["draft"] is not None:
             reorder_slots(StateBuffers([st["draft"]]), slots, beam_idx.to(slots.device))
@@ -233,7 +236,7 @@ def _following(cls):
 
     return type(cls)(cls.__name__, (cls,), {
         "__module__": cls.__module__, "__qualname__": cls.__qualname__, "__doc__": cls.__doc__, "plain": cls,
-        "reorder_cache": property(lambda self: _FollowBeams(self, self._nssm_st)),
+        "reorder_cache": property(lambda self: _FollowBeams(self, *self._nssm_st)),
         "__copy__": shallow, "__deepcopy__": deep, "__reduce_ex__": reduce})
 
 
@@ -242,7 +245,8 @@ def _follow_beams(layer, st) -> None:
     if hasattr(type(layer), "reorder_cache"):
         if not hasattr(layer, "_nssm_st"):
             layer.__class__ = _following(type(layer))
-        layer._nssm_st = st
+        st["prefill"] = object()         # whose states the pool holds: this layer's and its copies'
+        layer._nssm_st = (st, st["prefill"])
 
 
 def _dispatch(self, input_states, cache_params=None, attention_mask=None):

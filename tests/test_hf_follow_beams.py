@@ -87,3 +87,18 @@ def test_a_layer_can_be_pickled_and_saved(monkeypatch, tmp_path):
         first.reorder_cache(torch.tensor([1, 0, 3, 2]))
         assert first.rows.tolist() == [1, 0, 3, 2]
     assert st["slots"].tolist() == [3, 1, 0, 2] and isinstance(layer, Layer) and layer.reorder_cache.st is st
+
+
+def test_an_older_cache_leaves_the_pool_to_the_newer(monkeypatch):
+    """A mixer has one pool: after another cache's prefill it holds that cache's states."""
+    calls = []
+    old, new, st = Layer(), Layer(), _state(calls, monkeypatch)
+    hf._follow_beams(old, st)
+    kept = copy.deepcopy(old)
+    hf._follow_beams(new, st)
+    for layer in (old, kept):
+        layer.reorder_cache(torch.tensor([1, 0]))      # fewer rows than the pool's, too
+        assert layer.rows.tolist() == [1, 0]
+    assert not calls and st["slots"].tolist() == [3, 1, 0, 2]
+    copy.deepcopy(new).reorder_cache(torch.tensor([1, 1, 2, 0]))
+    assert len(calls) == 1 and st["slots"].tolist() == [1, 1, 0, 3]
