@@ -207,7 +207,11 @@ class _FollowBeams:
             return
         slots = st["slots"]
         if st["draft"] is not None:
-            reorder_slots(StateBuffers([st["draft"]]), slots, beam_idx.to(slots.device))
+            bufs = st.get("draft_bufs")
+            if bufs is None or bufs.tensors[0] is not st["draft"]:
+                bufs = st["draft_bufs"] = StateBuffers([st["draft"]])
+                bufs.status = st["pool"].status        # the pool's check_status() tells of both
+            reorder_slots(bufs, slots, beam_idx.to(slots.device))
         st["slots"] = reorder_slots(st["pool"], slots, beam_idx.to(slots.device))
 
 

@@ -102,3 +102,28 @@ def test_an_older_cache_leaves_the_pool_to_the_newer(monkeypatch):
     assert not calls and st["slots"].tolist() == [3, 1, 0, 2]
     copy.deepcopy(new).reorder_cache(torch.tensor([1, 1, 2, 0]))
     assert len(calls) == 1 and st["slots"].tolist() == [1, 1, 0, 3]
+
+
+def test_moves_of_the_draft_report_to_the_pool(monkeypatch):
+    """The draft's buffers are described once and share the pool's status word."""
+    made, calls = [], []
+
+    class Buffers:
+        def __init__(self, tensors):
+            self.tensors, self.status = tensors, "its own"
+            made.append(self)
+
+    class Pool:
+        status = "the pool's"
+
+    monkeypatch.setattr(hf, "StateBuffers", Buffers)
+    layer, st = Layer(), _state(calls, monkeypatch)
+    st["pool"], st["draft"] = Pool(), torch.zeros(4, 2)
+    hf._follow_beams(layer, st)
+    for _ in range(3):
+        layer.reorder_cache(torch.tensor([1, 0, 2, 3]))
+    assert len(made) == 1 and made[0].tensors[0] is st["draft"] and made[0].status is Pool.status
+    assert [c[0] for c in calls] == [made[0], st["pool"]] * 3
+    st["draft"] = torch.zeros(4, 2)          # a larger batch's prefill makes another
+    layer.reorder_cache(torch.tensor([1, 0, 2, 3]))
+    assert len(made) == 2 and made[1].tensors[0] is st["draft"]
