@@ -197,6 +197,18 @@ def device_index(*tensors) -> int:
     return dev
 
 
+def int32_list(t: torch.Tensor, name: str) -> torch.Tensor:
+    """``t`` as a contiguous int32 tensor; what int32 cannot hold becomes its largest or smallest value, which no
+    slot or row has, and is then reported like any value out of range."""
+    if t.dtype != torch.int32:
+        if t.is_floating_point() or t.dtype == torch.bool:
+            raise ValueError(f"{name} must hold integers, got {t.dtype}")
+        if t.dtype == torch.int64:
+            t = t.clamp(-1 << 31, (1 << 31) - 1)
+        t = t.to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
+
+
 def call(fn, dev: int, *args) -> None:
     """``fn(*args, stream)`` on device ``dev`` and its current stream."""
     if torch.cuda.current_device() == dev:

@@ -41,9 +41,7 @@ def _indices(idx, n, name):
         idx = idx.reshape(-1)
     if idx.shape[0] != n:
         raise ValueError(f"{name} has {idx.shape[0]} entries, expected {n}")
-    if idx.dtype != torch.int32 or not idx.is_contiguous():
-        idx = idx.to(torch.int32).contiguous()
-    return idx
+    return _lib.int32_list(idx, name)
 
 
 def gated_delta_state_update(state: torch.Tensor, q, k, v, g, beta, scale: float | None = None,

@@ -81,10 +81,7 @@ def _target(buffers):
 
 
 def _list(t, name, n=None):
-    if t.dtype != torch.int32 or not t.is_contiguous():
-        if t.is_floating_point() or t.dtype == torch.bool:
-            raise ValueError(f"{name} must hold integers, got {t.dtype}")
-        t = t.to(torch.int32).contiguous()
+    t = _lib.int32_list(t, name)
     rows = t.numel()
     if n is not None and rows != n:
         raise ValueError(f"{name} has {rows} entries, expected {n}")

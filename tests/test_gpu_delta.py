@@ -688,3 +688,15 @@ def test_scan_takes_states_that_grow(b, H, g, T):
     assert bool(torch.isfinite(y).all()) and _rel(y, yr) <= Y_TOL
     for t in range(0, T, 16):             # and of every stretch of tokens by itself
         assert _rel(y[:, t:t + 16], yr[:, t:t + 16]) <= Y_TOL, t
+
+
+def test_step_reports_slots_beyond_32_bits():
+    from nested_ssm_b200 import gated_delta_state_update
+    x, state, _ = _step_case(3, 9, 2, 2, 32, 64, torch.float32, seed=34)
+    slots = torch.tensor([3, (1 << 32) + 5, -(1 << 32)], device="cuda")
+    out = torch.zeros(3, 2, 32, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ref = _step_ref(x, state, slots, 64 ** -0.5, out, [0])
+    gated_delta_state_update(state, x["q"], x["k"], x["v"], x["g"], x["beta"], None, slots, out=out, status=status)
+    _check_step(state, out, ref)
+    assert int(status) == 1

@@ -339,3 +339,13 @@ def test_reorder_reports_a_slot_named_twice_without_moves():
     assert reorder_slots(bufs, _i32([[4, 7], [7, -1]]), _i32([[0, 1], [0, 1]])).tolist() == [[4, 7], [7, -1]]
     _same(t, want)
     assert int(bufs.status) == 8
+
+
+def test_slots_beyond_32_bits_are_reported():
+    from nested_ssm_b200 import StateBuffers, copy_slots
+    t = [torch.randn(8, 5, device="cuda")]
+    bufs = StateBuffers(t)
+    want = _apply(t, [(2, 6)], 0)
+    copy_slots(bufs, torch.tensor([2, 1 << 32, 3], device="cuda"), torch.tensor([6, 4, (1 << 32) + 5], device="cuda"))
+    _same(t, want)
+    assert int(bufs.status) == 1

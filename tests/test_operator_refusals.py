@@ -200,3 +200,22 @@ def test_delta_scan_refuses_too_many_blocks():
                                            "workspace_bytes": 1 << 62, "cu_seqlens": None})
     _err(_lib.load().nssm_delta_scan(C.byref(a), None))
     assert "too large" in _lib.load().nssm_last_error().decode()
+
+
+def test_indices_that_int32_cannot_hold_stay_out_of_range():
+    t = torch.tensor([3, -1, 1 << 32, (1 << 32) + 3, -(1 << 40), (1 << 31) - 1])
+    assert _lib.int32_list(t, "t").tolist() == [3, -1, (1 << 31) - 1, (1 << 31) - 1, -(1 << 31), (1 << 31) - 1]
+    same = torch.tensor([5, 6], dtype=torch.int32)
+    assert _lib.int32_list(same, "t") is same
+    assert _lib.int32_list(torch.tensor([200, 7], dtype=torch.uint8), "t").tolist() == [200, 7]
+    for bad in (torch.zeros(2), torch.zeros(2, dtype=torch.bool)):
+        with pytest.raises(ValueError, match="integers"):
+            _lib.int32_list(bad, "t")
+
+
+@pytest.mark.parametrize("idx", [torch.zeros(2), torch.zeros(2, dtype=torch.bool)])
+def test_slots_and_bounds_are_integers(idx):
+    with pytest.raises(ValueError, match="integers"):
+        _step(state_batch_indices=idx)
+    with pytest.raises(ValueError, match="integers"):
+        _scan(cu_seqlens=idx)
