@@ -16,6 +16,16 @@ from . import _lib
 from .pool import TieredSlotPool
 
 
+def _layers_overlap(row, slot_stride, slots, outer_stride, layers):
+    """Whether two slots of different layers share memory: the distance of a pair is least for the slots next to the
+    layers' distance."""
+    for n in range(1, layers):
+        k = n * outer_stride // slot_stride if slots > 1 else 0
+        if any(abs(n * outer_stride - m * slot_stride) < row for m in (k, k + 1) if m < slots):
+            return True
+    return False
+
+
 def _describe(tensors, slot_dim):
     """One ``nssm_slot_buffer`` per tensor."""
     bufs = (_lib.NssmSlotBuffer * len(tensors))()
@@ -28,6 +38,8 @@ def _describe(tensors, slot_dim):
             row *= size
         if t.stride(slot_dim) < row and t.shape[slot_dim] > 1:
             raise ValueError("the slots of a buffer overlap")
+        if slot_dim and _layers_overlap(row, t.stride(1), t.shape[1], t.stride(0), t.shape[0]):
+            raise ValueError("the layers of a buffer overlap")
         d.base, d.row_bytes, d.slot_stride = t.data_ptr(), row * es, t.stride(slot_dim) * es
         d.outer, d.outer_stride = (t.shape[0], t.stride(0) * es) if slot_dim else (1, 0)
     return bufs

@@ -219,3 +219,37 @@ def test_slots_and_bounds_are_integers(idx):
         _step(state_batch_indices=idx)
     with pytest.raises(ValueError, match="integers"):
         _scan(cu_seqlens=idx)
+
+
+def _strided(shape, strides):
+    return torch.as_strided(torch.zeros(4096), shape, strides)
+
+
+@pytest.mark.parametrize("t,fine", [
+    (torch.zeros(3, 4, 5), True),
+    (torch.zeros(4, 3, 5).transpose(0, 1), True),                 # layers inside a slot's row
+    (torch.zeros(6, 8, 5)[::2, ::2], True),
+    (torch.zeros(1, 4, 5).expand(3, 4, 5), False),                # one layer under three names
+    (torch.zeros(1, 4, 5), True),
+    (torch.zeros(3, 1, 5), True),
+    (_strided((3, 4, 5), (5, 5, 1)), False),                      # layer 1 begins at slot 1 of layer 0
+    (_strided((3, 1, 5), (4, 5, 1)), False),
+    (_strided((2, 4, 5), (17, 10, 1)), False),                    # 17 is 3 before slot 2
+    (_strided((2, 4, 5), (15, 10, 1)), True),                     # between the slots
+    (_strided((2, 4, 5), (35, 10, 1)), True),                     # behind them
+    (_strided((2, 4, 5), (34, 10, 1)), False),
+])
+def test_state_buffers_of_layers_that_share_memory(t, fine):
+    with pytest.raises(RuntimeError if fine else ValueError, match="CUDA" if fine else "overlap"):
+        StateBuffers([t], slot_dim=1)
+
+
+def test_layers_overlap_equals_a_count_of_addresses():
+    from nested_ssm_b200.slots import _layers_overlap
+    for row in (1, 3):
+        for s in range(row, 9):
+            for o in range(0, 30):
+                for S in (1, 2, 4):
+                    for L in (1, 2, 3):
+                        at = [i * o + j * s + e for i in range(L) for j in range(S) for e in range(row)]
+                        assert _layers_overlap(row, s, S, o, L) == (len(set(at)) < len(at)), (row, s, o, S, L)
