@@ -1,6 +1,7 @@
 // nssm_delta_step / nssm_delta_scan: argument checks and launches of the gated delta rule.
 #include <cuda_runtime.h>
 #include <math.h>
+#include <stdlib.h>
 
 #include "nssm_delta_chunk.cuh"
 
@@ -106,6 +107,8 @@ int nssm_delta_step(const nssm_delta_step_args* a, void* stream) {
   if (!al(a->state, 16) || (a->state_stride_s & 3)) return fail(NSSM_ERR_INVALID, "state must be 16-byte aligned");
   if (a->state_stride_s < (int64_t)a->nheads * a->headdim * a->dstate)
     return fail(NSSM_ERR_INVALID, "state_stride_s smaller than a slot");
+  if ((a->batch > 1 && llabs(a->out_stride_b) < a->headdim) || (a->nheads > 1 && llabs(a->out_stride_h) < a->headdim))
+    return fail(NSSM_ERR_INVALID, "rows of out share memory");
   nssm::DeltaStepParams p{};
   p.H = a->nheads; p.G = a->ngroups; p.P = a->headdim; p.S = a->num_slots;
   slices(p.P, (int64_t)a->batch * p.H, &p.ns, &p.rows);
@@ -161,6 +164,10 @@ int nssm_delta_scan(const nssm_delta_scan_args* a, void* stream) {
   const int64_t row = (int64_t)a->nheads * a->headdim * a->dstate;
   if (a->final_states && a->batch > 1 && a->final_stride_b < row)
     return fail(NSSM_ERR_INVALID, "final_stride_b smaller than a state");
+  const int64_t yrow = (int64_t)a->nheads * a->headdim;
+  if ((a->seqlen > 1 && llabs(a->y_stride_t) < yrow) ||
+      (!a->cu_seqlens && tok && a->batch > 1 && llabs(a->y_stride_b) < yrow))
+    return fail(NSSM_ERR_INVALID, "tokens of y share memory");
   if (ws_chunks(a->batch, a->seqlen, a->cu_seqlens != nullptr) > (1 << 30)) return fail(NSSM_ERR_INVALID, "batch * seqlen too large");
   nssm::DeltaScanParams p{};
   p.B = a->batch; p.T = a->seqlen; p.H = a->nheads; p.G = a->ngroups; p.P = a->headdim;

@@ -253,3 +253,21 @@ def test_layers_overlap_equals_a_count_of_addresses():
                     for L in (1, 2, 3):
                         at = [i * o + j * s + e for i in range(L) for j in range(S) for e in range(row)]
                         assert _layers_overlap(row, s, S, o, L) == (len(set(at)) < len(at)), (row, s, o, S, L)
+
+
+@pytest.mark.parametrize("kw", [dict(out_stride_b=0, out_stride_h=32), dict(out_stride_b=128, out_stride_h=0),
+                                dict(out_stride_b=16, out_stride_h=128)])
+def test_delta_step_refuses_rows_of_out_that_share_memory(kw):
+    a = _fill(_lib.NssmDeltaStepArgs(), **{**DELTA, "num_slots": 8, "state_stride_s": 8192, **kw})
+    _err(_lib.load().nssm_delta_step(C.byref(a), None))
+    assert b"share memory" in _lib.load().nssm_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(y_stride_t=0), dict(y_stride_t=64), dict(y_stride_b=0)])
+def test_delta_scan_refuses_tokens_of_y_that_share_memory(kw):
+    a = _fill(_lib.NssmDeltaScanArgs(), **{**DELTA, "seqlen": 10, "q_stride_b": 1280, "q_stride_t": 128, "k_stride_b": 1280,
+                                           "k_stride_t": 128, "v_stride_b": 1280, "v_stride_t": 128, "y_stride_b": 1280,
+                                           "y_stride_t": 128, "final_stride_b": 8192, "init_stride_b": 8192,
+                                           "cu_seqlens": None, "workspace_bytes": 1 << 30, **kw})
+    _err(_lib.load().nssm_delta_scan(C.byref(a), None))
+    assert b"share memory" in _lib.load().nssm_last_error()
