@@ -24,7 +24,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_out: int | None 
 
     A logit that is not finite counts as masked (-inf).  Candidates of one beam rank by logit, then by
     the lower token; those of different beams by total (in 64 bits), then by the lower beam.  Masked
-    candidates are returned, with a score of -inf, only when there are no others."""
+    candidates are returned, with a score of -inf, only when there are no others.  Totals are formed as
+    (score + logit) - lse: a beam whose every logit is a finite mask of 1e16 and more loses its score beside
+    them, so a beam without tokens is masked with -inf."""
     if logits.dim() != 3 or scores.shape != logits.shape[:2]:
         raise ValueError(f"logits [b, K, V] and scores [b, K] expected, got {tuple(logits.shape)} and {tuple(scores.shape)}")
     b, K, V = logits.shape

@@ -1,7 +1,7 @@
 // Beam search's selection: one pass over the logits (sum of exponentials and the nout best of
 // each part of a row), then a merge per prompt.  The logits are read once: 64 x 8 rows of 131072 bf16
-// (134 MB) take 46 us, 38 of them the pass at 3.5 TB/s, which is bound by instruction issue (58 %):
-// an exponential, two conversions and two maxima a value.
+// (134 MB) take 51 us, 42 of them the pass at 3.2 TB/s, which is bound by instruction issue (51 % of
+// the slots) and by barriers: an exponential, two conversions and two maxima a value.
 //
 // Precision: the exponentials are 2^x to 2^-22 of themselves, a thread's and a part's sums fp32, parts are joined
 // and totals formed in 64 bits, (score + x) - lse.
@@ -487,9 +487,10 @@ namespace {
 
 using nssm_host::fail;
 
-// CTAs of a row: about two waves of the call's CTAs over the SMs (three fit on one), as few as that
-// allows: a part's first step pays for the bound, and every part leaves nout candidates to the
-// merge (64 x 8 rows of 131072: 48 us with two waves, 54 with four, 68 with six).
+// CTAs of a row: about two waves of the call's CTAs over B200's 148 SMs (three of the bf16 pass fit on one,
+// four of the fp32 pass), as few as that allows: a part's first step pays for the bound, and every part
+// leaves nout candidates to the merge (64 x 8 rows of 131072, at an earlier step: 48 us with two waves, 54
+// with four, 68 with six; 51 us now).  The workspace query, which needs no device, uses the same number.
 void row_parts(int64_t rows, int V, int bf16, int* splits, int* steps) {
   const int per = nssm::kBeamThreads * nssm::kVecs * (bf16 ? 8 : 4);
   const int all = (int)(((int64_t)V + (bf16 ? 7 : 3) + per - 1) / per);   // a row may begin inside its first piece

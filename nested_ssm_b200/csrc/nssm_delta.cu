@@ -32,7 +32,7 @@ int check_dims(int H, int G, int P, int N) {
 }
 
 // State rows of one head over CTAs of 4 threads a row: at most 40 rows, and 16 where the whole
-// call would otherwise not give every SM two CTAs (one row of 32 heads of 128: 2.8 us either way; 448
+// call would otherwise not give every one of B200's 148 SMs two CTAs (one row of 32 heads of 128: 2.8 us either way; 448
 // rows of 128 heads: 765 against 792 us).
 void slices(int P, int64_t heads, int* ns, int* rows) {
   *ns = (P + nssm::kStepRows - 1) / nssm::kStepRows;

@@ -63,9 +63,9 @@ __device__ __forceinline__ float sum4(float v) {
 // pieces of it in flight at once (128 bytes a thread at N = 128, which is what keeps HBM busy).  k and
 // q of the head wait in shared memory.  The output is read off the old state,
 // y = scale (e^g S q + u (k.q)), so that S k and S q reduce together.  448 rows of 128 heads of 80
-// (4.7 GB): 765 us, 6.2 TB/s with four CTAs of 40 rows an SM (one loads while another computes);
-// 838 us with two of 80, 827 with five at 80 registers; 1883 with 8 lanes a row, half the bytes in
-// flight and k and q in registers.  Rows are compared with the earlier rows' slots while the state is
+// (4.7 GB): 782 to 823 us from box to box, 5.7 to 6.0 TB/s, with four CTAs of 40 rows an SM (one loads
+// while another computes).  Timed on one box: 765 us so, 838 with two CTAs of 80 rows, 827 with five
+// at 80 registers; 1883 with 8 lanes a row, half the bytes in flight and k and q in registers.  Rows are compared with the earlier rows' slots while the state is
 // on its way.
 constexpr int kStepRows = 40, kStepThreads = 4 * kStepRows;
 template <int N>

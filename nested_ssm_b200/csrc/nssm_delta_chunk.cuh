@@ -14,17 +14,19 @@
 // S Q^T, U^T M^T, U'^T K), so S, r and u go from one product to the next inside a warp's
 // registers, and warps share only the K, Q, T and M tiles.  The chain of a chunk never leaves the
 // register file; on tcgen05 each of its four dependent products would cross tensor memory twice,
-// with the same conversions between, for a 128-row tile that most headdims do not fill.
+// with the same conversions between (not built: with S transposed, dstate on the 128 lanes and the
+// headdim as N, its rate is four times this one's).
 //
-// What bounds it.  Of 2 x 8192 tokens of 32 heads of 128 (492 us; input and output alone 63 us) the
-// walk takes 390: a chain of 256 chunks, one warp on each quarter of 128 SMs, 2700 cycles a chunk, of
-// them 1170 mma (146 products of 8 cycles a quarter; 82 more, with y, in the helper warp).  Of
-// 8 x 2048 tokens of 128 heads of 80 (933 us; 128 us) it takes 760: two warps a quarter, 228 products
-// a chunk, the tensor pipe 55 to 73 % busy, 4.3 waves of CTAs.  Not kept: chunks of 64 (T costs four
-// times as much a chunk: 1703 against 937 us), bf16 operands in three pieces (316 products a chunk
-// against 184 at the same precision of y; two pieces leave 3.6e-6 in the state), splitting the columns of S over two or four warps
-// (the part of a chunk that is not split and the exchange take more than is won: 489 -> 619 us), V by
-// one small bulk copy a row (they cost the walk more than its arithmetic).
+// What bounds it.  Of 2 x 8192 tokens of 32 heads of 128 (555 us; input and output alone 63 us) the
+// walk takes 446: a chain of 256 chunks, one warp on each quarter of 128 SMs, 1.74 us a chunk (3400
+// cycles at 1965 MHz), of them 1170 cycles mma (146 products of 8 cycles a quarter) beside 660 of the
+// helper warp with y (82 products).  Of 8 x 2048 tokens of 128 heads of 80 (1090 us; 128 us) it takes
+// 900: two warps a quarter, 228 products a chunk, the tensor pipe 58 % busy (4 x 512 tokens), 4.3
+// waves of CTAs.  Not kept (timed against 490 and 937 us, before y had two-piece operands): chunks of
+// 64 with T by one substitution (four times the cost a chunk: 1703 us), bf16 operands in three pieces
+// (316 products a chunk against 184; two pieces leave 3.6e-6 in the state), splitting the columns of S
+// over two or four warps (the part of a chunk that is not split and the exchange take more than is won:
+// 619 us), V by one small bulk copy a row (they cost the walk more than its arithmetic).
 //
 // Precision.  The state is fp32, and its products are to be as good: an fp32 operand goes in as two
 // fp16 values (11 bits each, the second holds what the first leaves), scaled by a power of two that
@@ -173,9 +175,9 @@ __device__ __forceinline__ int seq_chunks(const DeltaScanParams& p, int i) {
 }
 
 // ---------------------------------------------------------------- T and M of every chunk
-// Bound by latency (a CTA loads, converts, multiplies, then solves) and by issue: 170 us for 8 x 2048
-// tokens of 128 heads, 104 for 2 x 8192 of 32 heads, which move 0.41 and 0.35 GB.  Seven CTAs an SM;
-// with five 174 and 116, with four 178 and 128.
+// Bound by latency (a CTA loads, converts, multiplies, then solves) and by issue (58 %): 191 us for
+// 8 x 2048 tokens of 128 heads, 109 for 2 x 8192 of 32 heads, which write 0.51 and 0.25 GB.  Seven CTAs
+// an SM (with one piece of M: 170 and 104 us; with five CTAs 174 and 116, with four 178 and 128).
 // CTA: one chunk and key group, 4 warps.  k.k and q.k come from the tensor cores once per group
 // (products of bf16 values, fp32 sums); then a warp takes a head at a time, a lane a token row:
 // row i of T solves T (I + A) = I from column i down in fp32 (a backward substitution over A's
@@ -448,13 +450,14 @@ struct ChunkSmem {
 
 // A CTA takes four consecutive tiles of the heads of one key group, which share K and Q; they may
 // belong to different heads.  Two CTAs (up to 255 registers a thread) put two warps on each quarter
-// of an SM, whatever the headdim; three CTAs of 168 registers were slower (844 against 819 us for
-// 8 x 2048 tokens of 128 heads of 80).
+// of an SM, whatever the headdim (one CTA where it is 16 and dstate 128: four heads' T and M take
+// 143 KB); three CTAs of 168 registers were slower (844 against 819 us for 8 x 2048 tokens of 128
+// heads of 80, when those took 937 in all).
 //
 // HELP: where a call has no more CTAs than SMs, one warp on each quarter would do all of a chunk's
 // work in turn.  y is not part of the chain from chunk to chunk, so a second warp computes it from
 // the operands that the first one hands over (one prompt of 4096 tokens, 32 heads of
-// 128: the walk 205 against 244 us).
+// 128, before y had two-piece operands: the walk 205 against 244 us).
 template <int N, bool HELP>
 __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta_chunk_kernel(const DeltaChunkParams p) {
   using L = ChunkSmem<N>;
@@ -466,7 +469,7 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
   int s = blockIdx.y, batch, t0, len;
   if (p.s.cu && p.s.B > 1 && p.s.B <= kSorted) {
     // the longest sequences first: CTAs start in this order, and the last ones to start should be short
-    // (24 prompts of 35 to 700 tokens, 32 heads of 128: 206 against 231 us)
+    // (24 prompts of 35 to 700 tokens, 32 heads of 128, with one-piece operands of y: 206 against 231 us)
     __shared__ int lens[kSorted], chosen;
     for (int i = tid; i < p.s.B; i += blockDim.x) lens[i] = delta_seq(p.s, i, &batch, &t0, &len) ? len : 0;
     __syncthreads();
