@@ -431,8 +431,9 @@ NSSM_API size_t nssm_sizeof_delta_step_args(void);
  * tokens (the _b strides of the inputs are not used); tokens outside every sequence are not
  * read, and their y is not written.  Sequences with bad bounds are skipped and touch no other.  Sequences must not
  * overlap: the y of shared tokens is either one's, and those without room in the workspace are skipped.  g may be
- * -inf and above 0; any other value of
- * a sequence that is not finite reaches every y of its block of 32 tokens, and the state.  q, k, v, y bf16; token strides multiples of 8 elements,
+ * -inf and above 0; any other value of a sequence that is not finite reaches every y of its block of 32 tokens,
+ * and the state.  What a head writes in a block, beta (v - S k), is held relative to the block's largest: with fewer
+ * than 22 bits below 2^-17 of it, as nothing below 2^-40.  q, k, v, y bf16; token strides multiples of 8 elements,
  * bases 16-byte aligned; (group, dstate) and (head, headdim) packed; heads of g and beta packed. */
 typedef struct {
   int32_t batch;          /* sequences                                               */

@@ -799,7 +799,8 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
     // state before its second pieces run into fp16's smallest values, and is seldom 2^10 above it.  (Where
     // every first piece is zero, |S| may be just below 2^-24.)
     // O has a scale of its own, so.s, with so.s |u~| below 2^15: a chunk may read a state and forget it that is far
-    // above what it leaves.  Where S is more than 2^64 above u~, u~ loses bits instead of O leaving fp32.
+    // above what it leaves.  Where S is more than 2^64 above u~, u~ loses bits instead of O leaving fp32.  No
+    // factor between two scales leaves fp32: each scale is at most 2^104 above the largest of what it is applied to.
     const float inv_u = fr.inv * fac[5 * kC];
     float umax = 0.0f, wmax = 0.0f;
     float2 et[kTiles];
@@ -812,8 +813,9 @@ __global__ void __launch_bounds__(kWarps * (HELP ? 64 : 32), HELP ? 1 : 2) delta
     }
     const float egc = fac[5 * kC + 1];
     const float bs = su.inv * fmaxf(fmaxf(__low2float(smax), __high2float(smax)), 0x1p-24f);
-    const Pow2 sn = warp_scale(fmaxf(2.001f * egc * bs, 0x1p15f * inv_u * wmax));
-    const Pow2 so = warp_scale(fmaxf(0x1p-64f * fac[5 * kC + 2] * bs, inv_u * umax));
+    const float bu = inv_u * fmaxf(umax, 0x1p-24f);
+    const Pow2 sn = warp_scale(fmaxf(2.001f * egc * bs, 0x1p15f * fmaxf(inv_u * wmax, 0x1p-64f * bu)));
+    const Pow2 so = warp_scale(fmaxf(0x1p-64f * fac[5 * kC + 2] * bs, bu));
     const float os = su.inv * so.s, uo = inv_u * so.s, us = inv_u * sn.s, es = egc * su.inv * sn.s;
     su = sn;
 #pragma unroll

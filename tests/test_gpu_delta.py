@@ -700,3 +700,22 @@ def test_step_reports_slots_beyond_32_bits():
     gated_delta_state_update(state, x["q"], x["k"], x["v"], x["g"], x["beta"], None, slots, out=out, status=status)
     _check_step(state, out, ref)
     assert int(status) == 1
+
+
+@_both_walks()
+@pytest.mark.parametrize("size", [1e11, 1e18])
+@pytest.mark.parametrize("decay", [-50.0, -100.0, -160.0])
+def test_scan_erases_and_forgets_a_large_state_in_one_block(b, H, size, decay):
+    """A block whose first u are those of a state far above the values (it erases along its keys) and decay to
+    nothing within it, and whose last tokens write little or nothing."""
+    from nested_ssm_b200 import gated_delta_chunk_scan
+    d = _inputs(b, 100, H, 1, 32, 64, seed=35)
+    d["s0"] *= size
+    d["g"][:, 20] = decay
+    d["beta"][:, 20:40] = 0.0
+    x = [d[n] for n in ("q", "k", "v", "g", "beta")]
+    y, S = gated_delta_chunk_scan(*x, initial_states=d["s0"], return_final_states=True)
+    yr, Sr = OD.gated_delta_scan(*x, S0=d["s0"])
+    _check_y(y[:, :20], yr[:, :20], "before")
+    _check_y(y[:, 40:], yr[:, 40:], "behind")
+    _check_state(S, Sr)
