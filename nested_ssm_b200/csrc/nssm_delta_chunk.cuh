@@ -17,11 +17,11 @@
 // with the same conversions between (not built: with S transposed, dstate on the 128 lanes and the
 // headdim as N, its rate is four times this one's).
 //
-// What bounds it.  Of 2 x 8192 tokens of 32 heads of 128 (555 us; input and output alone 63 us) the
-// walk takes 446: a chain of 256 chunks, one warp on each quarter of 128 SMs, 1.74 us a chunk (3400
+// What bounds it.  Of 2 x 8192 tokens of 32 heads of 128 (551 us; input and output alone 63 us) the
+// walk takes 442: a chain of 256 chunks, one warp on each quarter of 128 SMs, 1.73 us a chunk (3400
 // cycles at 1965 MHz), of them 1170 cycles mma (146 products of 8 cycles a quarter) beside 660 of the
-// helper warp with y (82 products).  Of 8 x 2048 tokens of 128 heads of 80 (1090 us; 128 us) it takes
-// 900: two warps a quarter, 228 products a chunk, the tensor pipe 58 % busy (4 x 512 tokens), 4.3
+// helper warp with y (82 products).  Of 8 x 2048 tokens of 128 heads of 80 (1070 us; 128 us) it takes
+// 880: two warps a quarter, 228 products a chunk, the tensor pipe 58 % busy (4 x 512 tokens), 4.3
 // waves of CTAs.  Not kept (timed against 490 and 937 us, before y had two-piece operands): chunks of
 // 64 with T by one substitution (four times the cost a chunk: 1703 us), bf16 operands in three pieces
 // (316 products a chunk against 184; two pieces leave 3.6e-6 in the state), splitting the columns of S
@@ -35,8 +35,8 @@
 // token's largest lose bits).  The r of a chunk share one scale, as do its u: those more than 2^17 below a warp's
 // largest lose bits.  T, M and u go in as two pieces, so only products of two second pieces are
 // left out, 2^-22 of a product.  y is the fp32 sum rounded once to bf16 (single fp16 operands, 2^-12, in its
-// own products moved 3e-4 of it, and one value in thirty by a step; they take 504 against 557 us for 2 x 8192
-// tokens of 32 heads, 950 against 1086 for 8 x 2048 of 128).
+// own products moved 3e-4 of it, and one value in thirty by a step; they take 504 against 551 us for 2 x 8192
+// tokens of 32 heads, 950 against 1070 for 8 x 2048 of 128).
 #pragma once
 
 #include <cuda_fp16.h>
@@ -175,7 +175,7 @@ __device__ __forceinline__ int seq_chunks(const DeltaScanParams& p, int i) {
 }
 
 // ---------------------------------------------------------------- T and M of every chunk
-// Bound by latency (a CTA loads, converts, multiplies, then solves) and by issue (58 %): 191 us for
+// Bound by latency (a CTA loads, converts, multiplies, then solves) and by issue (58 %): 189 us for
 // 8 x 2048 tokens of 128 heads, 109 for 2 x 8192 of 32 heads, which write 0.51 and 0.25 GB.  Seven CTAs
 // an SM (with one piece of M: 170 and 104 us; with five CTAs 174 and 116, with four 178 and 128).
 // CTA: one chunk and key group, 4 warps.  k.k and q.k come from the tensor cores once per group

@@ -124,11 +124,12 @@ def gated_delta_chunk_scan(q, k, v, g, beta, scale: float | None = None, initial
     ``cu_seqlens[s]`` to ``cu_seqlens[s + 1]``; empty sequences keep their initial state, and
     the rows of ``out`` outside every sequence are left as they were.  Sequences whose bounds
     do not ascend inside ``[0, T]`` are skipped and set bit 3 of the int32 ``status``; they touch no
-    other.  Sequences must not overlap.  Otherwise n == b.  ``initial_states [n, H, P, N]`` fp32 (zeros without them); ``final_states`` may be the
-    same tensor.  ``g`` may be ``-inf`` (the state is forgotten) and above 0 (it grows); any other value of a sequence that
-    is not finite reaches every output of its 32-token block, those before it too, and the state.
-    What a head writes in a block, beta (v - S k), is held relative to the block's largest: with fewer
-    than 22 bits below 2^-17 of it, as nothing below 2^-40."""
+    other.  Sequences must not overlap.  Otherwise n == b.  ``initial_states [n, H, P, N]`` fp32
+    (zeros without them); ``final_states`` may be the same tensor.  ``g`` may be ``-inf`` (the state
+    is forgotten) and above 0 (it grows); any other value of a sequence that is not finite reaches
+    every output of its 32-token block, those before it too, and the state.  What a head writes in a
+    block, beta (v - S k), is held relative to the block's largest: with fewer than 22 bits below
+    2^-17 of it, as nothing below 2^-40."""
     qs, vs = q.shape, v.shape
     if len(qs) != 4 or k.shape != qs or len(vs) != 4:
         raise ValueError("q / k [b, T, G, N], v [b, T, H, P], g / beta [b, T, H] expected")
